@@ -2,11 +2,11 @@
 
 A cache is a tensor of pages. A page holds `page` tokens of every head; a head's part of it is
 
-    K codes [page][D/2] | V codes [page/4][16][4][D/32 bytes] | K scales [page][D/32] | V scales [page][D/32]
+    K codes [page][D/2] | V codes [page/4][16][4][D/32 bytes] | K scales [page][D/32] | V scales [page/4][D/32][4]
 
 with D = head_dim padded to 64, 128 or 256. Codes are E2M1 (low nibble = even element), scales one exponent byte for each
-32 elements of a token's row. The V codes of four tokens lie together in 16 pieces of D/16 elements, so that one load of the
-attention's value product takes four tokens of its columns.
+32 elements of a token's row. The V codes of four tokens lie together in 16 pieces of D/16 elements, their scales block by
+block, so that one load of the attention's value product takes four tokens of its columns.
 
 `own` is set from outside: False computes every operator with elementary torch operations, True calls the framework."""
 import math
@@ -150,7 +150,7 @@ def _parts(case, heads):
     """Views of a head's bytes [..., head bytes] as (K codes, V codes, K scales, V scales)."""
     p, w = case["page"], _width(case["head_dim"])
     k, v, ks, vs = heads.split((p * w // 2, p * w // 2, p * w // 32, p * w // 32), -1)
-    return (k.unflatten(-1, (p, w // 2)), v.unflatten(-1, (p // 4, 16, 4, w // 32)), ks.unflatten(-1, (p, w // 32)), vs.unflatten(-1, (p, w // 32)))
+    return (k.unflatten(-1, (p, w // 2)), v.unflatten(-1, (p // 4, 16, 4, w // 32)), ks.unflatten(-1, (p, w // 32)), vs.unflatten(-1, (p // 4, w // 32, 4)))
 
 
 def _write_slots(case, cache, k, v, slots):
@@ -163,7 +163,7 @@ def _write_slots(case, cache, k, v, slots):
     ks[page, :, at] = scales
     codes, scales = _encode(v)
     vc[page, :, at // 4, :, at % 4] = codes.unflatten(-1, (16, -1))
-    vs[page, :, at] = scales
+    vs[page, :, at // 4, :, at % 4] = scales
 
 
 def _read_slots(case, cache, slots):
@@ -171,14 +171,14 @@ def _read_slots(case, cache, slots):
     p = case["page"]
     kc, vc, ks, vs = _parts(case, cache)
     page, at = slots // p, slots % p
-    return (_decode(kc[page, :, at], ks[page, :, at]), _decode(vc[page, :, at // 4, :, at % 4].flatten(-2), vs[page, :, at]))
+    return (_decode(kc[page, :, at], ks[page, :, at]), _decode(vc[page, :, at // 4, :, at % 4].flatten(-2), vs[page, :, at // 4, :, at % 4]))
 
 
 def _read_pages(case, cache, tables):
     """(keys, values) [requests, heads, tokens, D] of whole block tables [requests, pages]."""
     kc, vc, ks, vs = _parts(case, cache[tables])
     k = _decode(kc, ks)                                                   # [requests, pages, heads, page, D]
-    v = _decode(vc.transpose(-2, -3).flatten(-2).flatten(-3, -2), vs)
+    v = _decode(vc.transpose(-2, -3).flatten(-2).flatten(-3, -2), vs.transpose(-1, -2).flatten(-3, -2))
     return k.transpose(1, 2).flatten(2, 3), v.transpose(1, 2).flatten(2, 3)
 
 
@@ -367,7 +367,7 @@ def _selected_plain(s):
     kc, vc, ks, vs = _parts(case, s["cache"])
     head = torch.arange(h, device="cuda")[:, None, None]
     key = _decode(kc[page, head, at], ks[page, head, at])                                          # [h, n, k, D]
-    val = _decode(vc[page, head, at // 4, :, at % 4].flatten(-2), vs[page, head, at])
+    val = _decode(vc[page, head, at // 4, :, at % 4].flatten(-2), vs[page, head, at // 4, :, at % 4])
     q = torch.nn.functional.pad(s["q"].float(), (0, w - d)).unflatten(1, (h, g)).transpose(0, 1) / math.sqrt(d)
     score = torch.matmul(q, key.transpose(-1, -2).contiguous())                                    # [h, n, g, k]
     out, lse = _softmax_sum(score, seen[:, :, None], val)
@@ -480,7 +480,7 @@ def _head64(case, cache, h, pages, at):
     key_at = base + t * (w // 2) + e // 2
     val_at = base + half + (t // 4) * (2 * w) + (e // piece) * (piece * 2) + (t % 4) * (piece // 2) + (e % piece) // 2
     key_s = base + 2 * half + t * (w // 32) + e // 32
-    val_s = key_s + p * (w // 32)
+    val_s = base + 2 * half + p * (w // 32) + (t // 4) * (w // 8) + (e // 32) * 4 + t % 4
     shift = (4 * (e % 2)).to(torch.uint8)
     return (_value64((flat[key_at] >> shift) & 15, flat[key_s]), _value64((flat[val_at] >> shift) & 15, flat[val_s]))
 
