@@ -429,6 +429,90 @@ int zvdb_hip_search_graph_sharded_dev(zvdb_hip_index *h, zvdb_hip_comm *c, const
 int zvdb_hip_timing_enable(zvdb_hip_index *h, int enable);
 int zvdb_hip_timing_read(zvdb_hip_index *h, double *out_total_ms, uint32_t *out_launches);
 
+/* ---- 4-bit key/value cache (extension; no reference symbol) ---------------- */
+/* What a language model reads behind the rows of an index: keys and values of its tokens, held in 4 bits, and attention over
+ * them -- over whole requests, or over the rows whose ids a search of this library returned.  The calls hold no state: the
+ * cache, its block tables and every length are the caller's device memory, every call is a _dev call (device pointers, the
+ * caller's stream, nothing allocated, nothing synchronised: a captured call replays).  All pointers of a call are memory of
+ * ONE device, which need not be the current one, and so is the stream's; arrays of rows are 16-byte aligned.
+ *
+ * Cache: `pages` pages of zvdb_hip_kv_page_bytes each, one after the other.  A page holds page_size tokens of every head; of
+ * each head, with D = head_dim padded to 64, 128 or 256 (padding holds zeros) and NB = D / 32:
+ *     K codes [page_size][D/2] | V codes [page_size/4][16][4][NB] | K scales [page_size][NB] | V scales [page_size/4][NB][4]
+ * Codes are OCP E2M1, the low nibble the even element; V's row is cut into 16 pieces of 2 NB elements, and the pieces and the
+ * scales of four tokens lie side by side.  A block of 32 elements has one scale byte b: 2^(b - 127), the power of two at or
+ * under the block's largest magnitude over 4, the next one from 7/4 of it on, within 2 <= b <= 252; 255: the block held a NaN
+ * or an infinity and reads back as NaN.  A code is the nearest of x / scale, ties to even, saturating at 6.
+ *
+ * Slot of a token: page * page_size + place in the page; UINT64_MAX (any slot outside the cache): none.
+ * Block table: row i of d_tables (u32, table_stride entries) holds the pages of request i in order; an entry that is no page
+ * (>= pages) hides its tokens. */
+typedef struct zvdb_hip_kv_layout {
+    uint32_t abi_version; /* ZVDB_HIP_ABI_VERSION */
+    uint32_t head_dim;    /* a multiple of 8, 8 .. 256 */
+    uint32_t kv_heads;    /* 1 .. 1024 */
+    uint32_t page_size;   /* tokens: 16, 32, 64, 128 or 256 */
+    uint64_t pages;
+} zvdb_hip_kv_layout;
+
+enum zvdb_kv_type { ZVDB_KV_F32 = 0, ZVDB_KV_BF16 = 1 };
+
+/* Bytes of one page, all heads: page_size * kv_heads * (D + D/16). */
+int zvdb_hip_kv_page_bytes(const zvdb_hip_kv_layout *layout, uint64_t *out_bytes);
+
+enum zvdb_kv_plan_status {
+    ZVDB_KV_PLANNED = 0,
+    ZVDB_KV_OUT_OF_PAGES = 1,    /* the ring holds fewer pages than the batch needs */
+    ZVDB_KV_TABLE_TOO_SHORT = 2, /* a request outgrows table_stride pages (or 2^31 - 1 tokens) */
+    ZVDB_KV_SLOTS_TOO_FEW = 3    /* more new tokens than slot_cap */
+};
+
+/* Gives the new tokens of n requests (n <= 16384) their pages and slots, on the device.  Request i holds d_lengths[i] tokens (u32)
+ * and gets d_new[i] more (0 is fine).  Free pages wait in a ring, d_ring[ring_size] u32, between the counts
+ * d_cursor[0] (taken so far) and d_cursor[1] (given so far; u64): page number c of the ring is d_ring[c % ring_size].  The caller
+ * returns pages by writing them behind `given`.  Pages are taken in the order of the requests.  Writes:
+ *   d_tables        the new entries only (the others stay as they are)
+ *   d_starts        u32[n + 1]: first new token of each request; d_starts[n] = their number
+ *   d_slots         u64[slot_cap]: slot of each new token, request by request; UINT64_MAX behind the last one
+ *   d_out_lengths   u32[n], d_out_cursor u64[2]: both after the call (not the input arrays: every block reads those)
+ *   d_status        u32[4]: enum zvdb_kv_plan_status, pages needed, new tokens, 0
+ * All or nothing: with a status other than ZVDB_KV_PLANNED no page is taken, no table changes, lengths and cursor stay, d_starts is 0
+ * and every slot UINT64_MAX, so that the calls behind it do nothing. */
+int zvdb_hip_kv_plan_dev(const zvdb_hip_kv_layout *layout, const void *d_lengths, const void *d_new, uint32_t n, const void *d_ring,
+                         uint32_t ring_size, const void *d_cursor, void *d_tables, uint32_t table_stride, void *d_starts, void *d_slots,
+                         uint64_t slot_cap, void *d_out_lengths, void *d_out_cursor, void *d_status, void *stream);
+
+/* Writes the keys and values of n tokens ([kv_heads][head_dim] of `type`, k_stride / v_stride elements from one token to the next, a
+ * multiple of 8) into their slots.  Tokens without a slot are skipped.  A slot may be named once in a call. */
+int zvdb_hip_kv_append_dev(const zvdb_hip_kv_layout *layout, void *d_cache, const void *d_k, uint64_t k_stride, const void *d_v, uint64_t v_stride,
+                           uint32_t type, uint32_t n, const void *d_slots, void *stream);
+
+/* Reads rows back, widened exactly: d_k, d_v [n][kv_heads][head_dim] of `type` (either may be NULL); zeros where there is no slot. */
+int zvdb_hip_kv_read_dev(const zvdb_hip_kv_layout *layout, const void *d_cache, const void *d_slots, uint32_t n, void *d_k, void *d_v, uint32_t type, void *stream);
+
+/* Attention of new tokens over their requests, o = softmax(scale q K^T) V with fp32 sums.  d_q: [rows][q_heads][head_dim] of `type`,
+ * q_stride elements from one token to the next (a multiple of 8); request i has the rows d_starts[i] .. d_starts[i + 1] (at most
+ * max_new of them; d_starts as zvdb_hip_kv_plan_dev writes it) and d_lengths[i] tokens (at most max_length), its new ones included.
+ * Query head h reads key/value head h / (q_heads / kv_heads).  causal: the j-th of m new tokens sees the tokens before position
+ * length - m + j + 1; else all of them.  d_out [rows][q_heads][head_dim] of `type`, d_lse fp32 [rows][q_heads] (log of the sum of
+ * exponentials; NULL: not wanted).  A row that sees nothing gets 0 and -inf.  A NaN reaches the rows that see its token and no others.
+ * Rows behind d_starts[n] stay as they are.  max_new and max_length are bounds that the host knows: what exceeds them is not
+ * computed, or not seen.  With ZVDB_KV_BF16 the probabilities are rounded to bf16 for their product with V; with ZVDB_KV_F32 queries and
+ * probabilities keep 24 bits.  Same inputs, same bits.  The workspace (zvdb_hip_kv_attend_workspace for the same sizes, on the same
+ * kind of device) belongs to one call at a time. */
+int zvdb_hip_kv_attend_workspace(const zvdb_hip_kv_layout *layout, uint32_t type, uint32_t q_heads, uint32_t n, uint32_t rows, uint32_t max_new, uint32_t max_length,
+                                 uint64_t *out_bytes);
+int zvdb_hip_kv_attend_dev(const zvdb_hip_kv_layout *layout, const void *d_cache, const void *d_q, uint64_t q_stride, uint32_t type, uint32_t q_heads, uint32_t n,
+                           const void *d_starts, uint32_t rows, uint32_t max_new, const void *d_lengths, const void *d_tables, uint32_t table_stride,
+                           uint32_t max_length, float scale, uint32_t causal, void *d_workspace, uint64_t workspace_bytes, void *d_out, void *d_lse, void *stream);
+
+/* The same over selected tokens: row i (one per request) and key/value head h see the tokens d_ids[h][i][0 .. count) of request i
+ * (u64, k to a list; count = d_count[h][i], u32, NULL: k), as zvdb_hip_search_*_dev leaves them for an index over that head's keys.
+ * Ids that are not below d_lengths[i] are passed over (UINT64_MAX in unused places is); an id listed twice counts twice. */
+int zvdb_hip_kv_attend_selected_dev(const zvdb_hip_kv_layout *layout, const void *d_cache, const void *d_q, uint64_t q_stride, uint32_t type, uint32_t q_heads,
+                                    uint32_t n, const void *d_ids, const void *d_count, uint32_t k, const void *d_lengths, const void *d_tables,
+                                    uint32_t table_stride, float scale, void *d_out, void *d_lse, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

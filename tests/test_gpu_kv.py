@@ -1,0 +1,560 @@
+"""The 4-bit key/value cache on the GPU, against the plain 64-bit restatement in _kv_ref.py: pages and rows bit for bit, attention within
+bounds derived there."""
+import numpy as np
+import pytest
+
+import _kv_ref as ref
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def torch():
+    import torch
+    return torch
+
+
+def stream(torch):
+    return torch.cuda.current_stream().cuda_stream
+
+
+def as_type(torch, x, kind):
+    """The tensor of fp64 values x in a type, and the values it then holds."""
+    t = torch.from_numpy(np.ascontiguousarray(x)).to(torch.float32)
+    t = t.to(torch.bfloat16 if kind == "bf16" else torch.float32)
+    return t.cuda(), t.double().numpy()
+
+
+def kv_type(kind):
+    import zvdb_amd as zv
+    return zv.KV_BF16 if kind == "bf16" else zv.KV_F32
+
+
+# ---- plan -------------------------------------------------------------------------------------------------------------------------
+
+def run_plan(torch, lengths, new, ring, cursor, tables, page, pages, slot_cap):
+    import zvdb_amd as zv
+    lay = zv.KVLayout(head_dim=64, kv_heads=1, page_size=page, pages=pages)
+    n = len(lengths)
+    i32 = lambda x: torch.tensor(np.asarray(x, dtype=np.uint32).view(np.int32), device="cuda")
+    L, N, R, T = i32(lengths), i32(new), i32(ring), i32(tables)
+    C = torch.tensor(np.asarray(cursor, np.int64), device="cuda")
+    starts = torch.full((n + 1 + 3,), -7, dtype=torch.int32, device="cuda")
+    slots = torch.full((slot_cap + 3,), -7, dtype=torch.int64, device="cuda")
+    outl = torch.full((n + 3,), -7, dtype=torch.int32, device="cuda")
+    outc, status = torch.zeros(2, dtype=torch.int64, device="cuda"), torch.full((4,), -7, dtype=torch.int32, device="cuda")
+    lay.plan_dev(L.data_ptr(), N.data_ptr(), n, R.data_ptr(), len(ring), C.data_ptr(), T.data_ptr(), tables.shape[1], starts.data_ptr(), slots.data_ptr(),
+                 slot_cap, outl.data_ptr(), outc.data_ptr(), status.data_ptr(), stream(torch))
+    torch.cuda.synchronize()
+    h = lambda t: t.cpu().numpy()
+    assert (h(starts)[n + 1:] == -7).all() and (h(slots)[slot_cap:] == -7).all() and (h(outl)[n:] == -7).all()
+    return h(status), h(starts)[:n + 1], h(slots)[:slot_cap], h(outl)[:n], h(outc), h(T).view(np.uint32)
+
+
+def check_plan(torch, lengths, new, ring, cursor, tables, page, pages, slot_cap):
+    got = run_plan(torch, lengths, new, ring, cursor, tables, page, pages, slot_cap)
+    code, starts, slots, outl, outc, tab, need, total = ref.plan(lengths, new, ring, cursor, tables, page, pages, slot_cap)
+    assert got[0].tolist() == [code, min(need, 2**31 - 1), min(total, 2**31 - 1), 0]
+    assert np.array_equal(got[1], starts) and np.array_equal(got[2], slots)
+    assert np.array_equal(got[3].astype(np.int64) & 0xFFFFFFFF, np.asarray(outl)) and np.array_equal(got[4], np.asarray(outc))
+    assert np.array_equal(got[5], tab)
+    return code
+
+
+def plan_case(rng, n, top_len, top_new, page, extra=0):
+    lengths = rng.integers(0, top_len + 1, n)
+    new = rng.integers(0, top_new + 1, n)
+    held = int(sum(-(-c // page) for c in lengths))
+    pages = held + int(sum(-(-(c + a) // page) for c, a in zip(lengths, new))) + 5
+    order = rng.permutation(pages)
+    stride = int(max([1] + [-(-(c + a) // page) for c, a in zip(lengths, new)])) + extra
+    tables = np.full((n, stride), 0xFFFFFFFF, np.uint32)
+    at = 0
+    for i, c in enumerate(lengths):
+        m = -(-int(c) // page)
+        tables[i, :m] = order[at:at + m]
+        at += m
+    return lengths, new, order.astype(np.uint32), [held, pages], tables, pages
+
+
+@pytest.mark.parametrize("n,top_len,top_new,page", [(1, 0, 1, 16), (1, 40, 1, 16), (3, 50, 0, 16), (64, 500, 1, 16), (65, 100, 70, 32), (300, 90, 33, 64), (1025, 40, 9, 16),
+                                                    (2500, 300, 3, 256), (16384, 20, 2, 16), (7, 10, 4000, 128)])
+def test_plan(torch, n, top_len, top_new, page):
+    rng = np.random.default_rng(n * 7 + page)
+    lengths, new, ring, cursor, tables, pages = plan_case(rng, n, top_len, top_new, page, extra=n % 3)
+    total = int(new.sum())
+    for cap in {total, total + 1, 2 * total + 37}:
+        assert check_plan(torch, lengths, new, ring, cursor, tables, page, pages, cap) == 0
+
+
+def test_plan_of_no_request(torch):
+    assert check_plan(torch, [], [], np.arange(4, dtype=np.uint32), [1, 3], np.zeros((0, 1), np.uint32), 16, 4, 5) == 0
+
+
+def test_plan_wraps_round_the_ring(torch):
+    rng = np.random.default_rng(0)
+    ring = rng.permutation(11).astype(np.uint32)
+    tables = np.full((4, 3), 0xFFFFFFFF, np.uint32)
+    for taken in (0, 5, 10, 11, 2**33 + 9):
+        assert check_plan(torch, [0, 0, 0, 0], [17, 33, 1, 40], ring, [taken, taken + 11], tables, 16, 11, 91) == 0
+
+
+@pytest.mark.parametrize("why", ["pages", "given behind taken", "table", "too long", "slots"])
+def test_plan_is_all_or_nothing(torch, why):
+    ring, cursor, stride, cap = np.arange(20, dtype=np.uint32), [3, 9], 4, 100
+    lengths, new = [16, 5, 0], [16, 20, 33]  # 1 + 1 + 3 pages
+    if why == "pages":
+        cursor = [5, 9]
+    elif why == "given behind taken":
+        cursor = [9, 3]
+    elif why == "table":
+        stride = 2
+    elif why == "too long":
+        lengths[1], new[1] = 2**31 - 2, 2
+    else:
+        cap = 68
+    tables = np.arange(3 * stride, dtype=np.uint32).reshape(3, stride)
+    want = {"pages": 1, "given behind taken": 1, "table": 2, "too long": 2, "slots": 3}[why]
+    assert check_plan(torch, lengths, new, ring, cursor, tables, 16, 20, cap) == want
+
+
+def test_plan_of_entries_that_are_no_page(torch):
+    """A partly filled page that is none, and a ring entry that is none: the tokens there get no slot."""
+    tables = np.array([[7, 99, 0, 0], [1, 2, 0, 0]], np.uint32)
+    assert check_plan(torch, [20, 16], [3, 20], np.array([3, 50, 4], np.uint32), [1, 4], tables, 16, 8, 30) == 0
+
+
+# ---- append and read --------------------------------------------------------------------------------------------------------------
+
+def special_rows(rng, n, heads, d):
+    """Normal rows with the cases a block can be: zeros, ties, one large element, largest and smallest numbers, NaN, infinities."""
+    x = rng.standard_normal((n, heads, d)) * np.exp2(rng.integers(-6, 7, (n, heads, 1)))
+    x = x.reshape(n * heads, d)
+    for r in range(len(x)):
+        c, at = r % 13, 8 * (r % (d // 8))
+        if c == 1:
+            x[r] = 0
+        elif c == 2:
+            x[r] = rng.integers(-24, 25, d) * 0.25          # ties of the grid
+        elif c == 3:
+            x[r, at] = 3e38
+        elif c == 4:
+            x[r] = rng.standard_normal(d) * 2.0 ** -126
+        elif c == 5:
+            x[r, at] = np.nan
+        elif c == 6:
+            x[r, at + 7] = -np.inf
+        elif c == 7:
+            x[r] = 7.0 * np.sign(x[r])                       # 7/4 of a power of two: the scale doubles
+        elif c == 8:
+            x[r] = -0.0
+        elif c == 9:
+            x[r] = 6.999 * np.sign(x[r])
+        elif c == 10:
+            x[r] = rng.standard_normal(d) * 2.0 ** -140
+    return x.reshape(n, heads, d)
+
+
+@pytest.mark.parametrize("d,heads,page,n,kind", [(64, 1, 16, 1, "bf16"), (64, 3, 16, 37, "fp32"), (8, 2, 32, 21, "fp32"), (72, 2, 64, 33, "bf16"), (96, 4, 16, 50, "fp32"),
+                                                 (128, 8, 128, 29, "bf16"), (128, 1, 16, 100, "fp32"), (136, 3, 16, 17, "bf16"), (256, 2, 256, 65, "bf16"),
+                                                 (256, 1, 32, 40, "fp32")])
+def test_append_and_read_bit_for_bit(torch, d, heads, page, n, kind):
+    import zvdb_amd as zv
+    rng = np.random.default_rng(d + n)
+    pages = -(-n // page) + 3
+    lay = zv.KVLayout(head_dim=d, kv_heads=heads, page_size=page, pages=pages)
+    fill = rng.integers(0, 256, pages * lay.page_bytes, dtype=np.uint8)
+    cache = torch.from_numpy(fill.copy()).cuda()
+    slots = rng.permutation(pages * page)[:n].astype(np.int64)
+    slots[::9] = -1                      # no slot
+    if n > 4:
+        slots[4] = pages * page          # behind the cache
+    row = heads * d
+    ks, vs = row + 8, 2 * row + 16       # strides of their own, as in a fused projection's output
+    with np.errstate(over="ignore"):
+        (k, kx), (v, vx) = (as_type(torch, special_rows(rng, n, heads, d), kind) for _ in range(2))
+    kbuf, vbuf = torch.zeros(n * ks, dtype=k.dtype, device="cuda"), torch.zeros(n * vs, dtype=k.dtype, device="cuda")
+    kbuf.view(n, ks)[:, :row], vbuf.view(n, vs)[:, :row] = k.reshape(n, row), v.reshape(n, row)
+    s_dev = torch.from_numpy(slots).cuda()
+    lay.append_dev(cache.data_ptr(), kbuf.data_ptr(), ks, vbuf.data_ptr(), vs, kv_type(kind), n, s_dev.data_ptr(), stream(torch))
+    want, vals = fill.copy(), [np.zeros((n, heads, d)) for _ in range(2)]
+    for side, x in enumerate((kx, vx)):
+        for h in range(heads):
+            codes, scales, val = ref.encode_rows(x[:, h], d)
+            for i, s in enumerate(slots):
+                if 0 <= s < pages * page:
+                    ref.put(want, d, heads, page, int(s), h, codes[i], scales[i], side == 1)
+                    vals[side][i, h] = val[i]
+    assert np.array_equal(cache.cpu().numpy(), want)
+    for out in ("bf16", "fp32"):
+        ok, ov = (torch.full((n + 1, heads, d), 5.0, dtype=torch.bfloat16 if out == "bf16" else torch.float32, device="cuda") for _ in range(2))
+        lay.read_dev(cache.data_ptr(), s_dev.data_ptr(), n, ok.data_ptr(), ov.data_ptr(), kv_type(out), stream(torch))
+        for o, x in zip((ok, ov), vals):
+            assert np.array_equal(o.double().cpu().numpy()[:n], x, equal_nan=True) and (o[n] == 5.0).all()
+        only = torch.empty_like(ov)      # one of the two
+        lay.read_dev(cache.data_ptr(), s_dev.data_ptr(), n, 0, only.data_ptr(), kv_type(out), stream(torch))
+        assert np.array_equal(only[:n].double().cpu().numpy(), vals[1], equal_nan=True)
+        lay.read_dev(cache.data_ptr(), s_dev.data_ptr(), n, only.data_ptr(), 0, kv_type(out), stream(torch))
+        assert np.array_equal(only[:n].double().cpu().numpy(), vals[0], equal_nan=True)
+
+
+# ---- attention --------------------------------------------------------------------------------------------------------------------
+
+class Memory:
+    """A cache filled through append_dev, with the values that it then stands for; what no token wrote holds 0xFF (NaN scales)."""
+
+    def __init__(self, torch, rng, lengths, d, heads, page, kind="fp32", stride=None, pages_more=2, spoil=None):
+        import zvdb_amd as zv
+        self.torch, self.lengths, self.d, self.heads, self.page = torch, list(lengths), d, heads, page
+        need = [-(-x // page) for x in self.lengths]
+        self.pages = sum(need) + pages_more
+        self.lay = zv.KVLayout(head_dim=d, kv_heads=heads, page_size=page, pages=self.pages)
+        self.cache = torch.full((self.pages * self.lay.page_bytes,), 255, dtype=torch.uint8, device="cuda")
+        order = rng.permutation(self.pages)
+        self.stride = stride or max([1] + need)
+        self.tables = np.full((len(lengths), self.stride), 0xFFFFFFFF, np.uint32)
+        at = 0
+        slots = []
+        for i, x in enumerate(self.lengths):
+            self.tables[i, :need[i]] = order[at:at + need[i]]
+            at += need[i]
+            slots += [int(self.tables[i, p // page]) * page + p % page for p in range(x)]
+        t = len(slots)
+        self.first = np.concatenate(([0], np.cumsum(self.lengths))).astype(int)
+        k, v = rng.standard_normal((2, t, heads, d)) * 1.5
+        if spoil:
+            spoil(self, k, v)
+        (kt, kx), (vt, vx) = as_type(torch, k, kind), as_type(torch, v, kind)
+        self.k, self.v = (np.stack([ref.encode_rows(x[:, h], d)[2] for h in range(heads)], 1) if t else np.zeros((0, heads, d)) for x in (kx, vx))
+        s = torch.tensor(slots, dtype=torch.int64, device="cuda")
+        if t:
+            self.lay.append_dev(self.cache.data_ptr(), kt.data_ptr(), heads * d, vt.data_ptr(), heads * d, kv_type(kind), t, s.data_ptr(), stream(torch))
+
+    def rows_of(self, i):
+        return slice(self.first[i], self.first[i + 1])
+
+    def i32(self, x):
+        return self.torch.tensor(np.asarray(x, np.uint32).view(np.int32), device="cuda")
+
+
+def attend(mem, q, new, group, kind, causal, scale, lengths=None, tables=None, max_new=None, max_length=None, rows=None, lse=True, ws=None, q_stride=None):
+    torch = mem.torch
+    heads, d = mem.heads * group, mem.d
+    lengths = mem.lengths if lengths is None else lengths
+    starts = np.concatenate(([0], np.cumsum(new))).astype(int)
+    rows = starts[-1] if rows is None else rows
+    max_new, max_length = max(new) if max_new is None else max_new, max(lengths) if max_length is None else max_length
+    typ = kv_type(kind)
+    out = torch.full((rows + 2, heads, d), 77.0, dtype=q.dtype, device="cuda")
+    l = torch.full((rows + 2, heads), 77.0, device="cuda")
+    size = mem.lay.attend_workspace(typ, heads, len(new), rows, max_new, max_length)
+    if ws is None:
+        ws = torch.full((size,), 255, dtype=torch.uint8, device="cuda")
+    S, L, T = mem.i32(starts), mem.i32(lengths), mem.i32(mem.tables if tables is None else tables)
+    mem.lay.attend_dev(mem.cache.data_ptr(), q.data_ptr(), q_stride or heads * d, typ, heads, len(new), S.data_ptr(), rows, max_new, L.data_ptr(), T.data_ptr(),
+                       mem.stride, max_length, scale, causal, ws.data_ptr() if size else 0, size, out.data_ptr(), l.data_ptr() if lse else 0, stream(torch))
+    torch.cuda.synchronize()
+    return out.double().cpu().numpy(), l.double().cpu().numpy(), size
+
+
+def check_rows(mem, got, lse, qx, rows, group, kind, scale, visible):
+    """rows: (row, request); visible(row, request): the tokens of the request that the row sees, as a list of places."""
+    for r, i in rows:
+        see = visible(r, i)
+        for h in range(mem.heads * group):
+            kh, vh = mem.k[mem.rows_of(i)][see, h // group], mem.v[mem.rows_of(i)][see, h // group]
+            with np.errstate(invalid="ignore"):
+                o, l, bo, bl = ref.attend_row(qx[r, h], kh, vh, scale, kind)
+            if np.isnan(kh).any():
+                assert np.isnan(got[r, h]).all() and np.isnan(lse[r, h]), (r, h)
+                continue
+            bad = np.isnan(vh).any(0)
+            assert np.array_equal(np.isnan(got[r, h]), bad), (r, h)
+            assert (np.abs(got[r, h] - o)[~bad] <= bo[~bad]).all(), (r, h, np.abs(got[r, h] - o).max(), bo.max())
+            assert lse[r, h] == l or abs(lse[r, h] - l) <= bl, (r, h, lse[r, h], l, bl)
+
+
+def check_attend(torch, lengths, new, d, heads, group, page, kind, causal, seed=0, few=None, spoil=None, **kw):
+    rng = np.random.default_rng(seed + d + sum(lengths))
+    mem = Memory(torch, rng, lengths, d, heads, page, spoil=spoil)
+    rows, qh = sum(new), heads * group
+    q, qx = as_type(torch, 1.7 * rng.standard_normal((max(rows, 1), qh, d)), kind)
+    scale = 1.0 / np.sqrt(d)
+    got, lse, size = attend(mem, q, new, group, kind, causal, scale, **kw)
+    owner = np.repeat(np.arange(len(new)), new)
+    starts = np.concatenate(([0], np.cumsum(new))).astype(int)
+
+    def visible(r, i):
+        j = r - starts[i]
+        return slice(0, max(0, lengths[i] - new[i] + j + 1) if causal else lengths[i])
+
+    pick = range(rows) if few is None or rows <= few else sorted(set(rng.choice(rows, few, replace=False)) | {0, rows - 1})
+    check_rows(mem, got, lse, qx, [(r, owner[r]) for r in pick], group, kind, float(np.float32(scale)), visible)
+    assert (got[rows:] == 77.0).all() and (lse[rows:] == 77.0).all()  # rows behind the last are left as they were
+    return mem, q, got, lse, size
+
+
+@pytest.mark.parametrize("kind", ["bf16", "fp32"])
+@pytest.mark.parametrize("d,heads,group,page", [(64, 2, 1, 16), (64, 1, 7, 32), (80, 2, 3, 16), (128, 2, 4, 64), (128, 1, 16, 16), (96, 1, 33, 128), (256, 1, 5, 16), (200, 2, 2, 256)])
+def test_single_tokens(torch, kind, d, heads, group, page):
+    check_attend(torch, [1, 2, 15, 16, 17, 31, 32, 33, 100, 127, 129], [1] * 11, d, heads, group, page, kind, True)
+
+
+@pytest.mark.parametrize("kind", ["bf16", "fp32"])
+@pytest.mark.parametrize("d,heads,group,page", [(64, 1, 2, 16), (128, 2, 4, 16), (256, 1, 3, 64)])
+def test_long_contexts_are_split_and_joined(torch, kind, d, heads, group, page):
+    *_, size = check_attend(torch, [2500, 1, 1300], [1, 1, 1], d, heads, group, page, kind, True)
+    assert size > 0  # (the call was split)
+
+
+@pytest.mark.parametrize("kind", ["bf16", "fp32"])
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("d,heads,group,page", [(64, 2, 2, 16), (128, 1, 4, 32), (72, 1, 5, 16), (256, 1, 2, 64)])
+def test_prompts(torch, kind, causal, d, heads, group, page):
+    # prompts over nothing, over a cache, one that leaves rows empty (more new tokens than tokens), none at all, a request without tokens
+    check_attend(torch, [40, 300, 70, 0, 129, 0], [40, 77, 0, 3, 1, 0], d, heads, group, page, kind, causal, few=60)
+
+
+@pytest.mark.parametrize("kind", ["bf16", "fp32"])
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_prompts_of_many_rows(torch, kind, d):
+    check_attend(torch, [700, 333], [513, 200], d, 1, 3, 16, kind, True, few=40)
+
+
+def test_rows_without_tokens_get_zero_and_minus_infinity(torch):
+    for new in ([5, 1], [90, 2]):
+        mem, q, got, lse, _ = check_attend(torch, [2, 0], new, 64, 1, 1, 16, "bf16", True)
+        assert (got[:new[0] - 2] == 0).all() and np.isneginf(lse[:new[0] - 2]).all()
+        assert (got[new[0]:sum(new)] == 0).all() and np.isneginf(lse[new[0]:sum(new)]).all()
+
+
+@pytest.mark.parametrize("kind", ["bf16", "fp32"])
+@pytest.mark.parametrize("new", [1, 40])
+def test_pages_that_are_none_hide_their_tokens(torch, kind, new):
+    rng = np.random.default_rng(3)
+    lengths, d, heads, group, page = [100, 48, 1400], 64, 2, 2, 16
+    mem = Memory(torch, rng, lengths, d, heads, page)
+    hide = {0: [0, 3, 6], 1: [0, 1, 2], 2: [1, 2, 40, 87]}
+    tables = mem.tables.copy()
+    for i, ps in hide.items():
+        for n, p in enumerate(ps):
+            tables[i, p] = (mem.pages, 0xFFFFFFFF, 0x80000000)[n % 3]
+    q, qx = as_type(torch, rng.standard_normal((3 * new, heads * group, d)), kind)
+    got, lse, _ = attend(mem, q, [new] * 3, group, kind, True, 0.25, tables=tables)
+
+    def visible(r, i):
+        return np.array([t for t in range(lengths[i] - new + r % new + 1) if t // page not in hide[i]], dtype=int)
+
+    check_rows(mem, got, lse, qx, [(r, r // new) for r in range(3 * new)], group, kind, 0.25, visible)
+    assert (got[new:2 * new] == 0).all() and np.isneginf(lse[new:2 * new]).all()
+
+
+@pytest.mark.parametrize("kind", ["bf16", "fp32"])
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_a_nan_reaches_the_rows_that_see_it_and_no_others(torch, kind, d):
+    def spoil(mem, k, v):
+        v[30, 0, 33] = np.nan         # one block of one value
+        v[61, 1, 0] = np.inf
+        k[45, 1, d - 1] = -np.inf     # a key: everything of the rows that see it
+    check_attend(torch, [70], [64], d, 2, 2, 16, kind, True, spoil=spoil)
+    check_attend(torch, [70], [3], d, 2, 2, 16, kind, True, spoil=spoil)
+    check_attend(torch, [50], [40], d, 1, 2, 16, kind, False, spoil=lambda mem, k, v: v.__setitem__((30, 0, 33), np.nan))
+
+
+def test_scores_of_any_size(torch):
+    """Large scores, rows whose maximum moves late, all scores equal, all far below zero."""
+    def spoil(mem, k, v):
+        k[:] = 0
+        k[10:, :, 0] = 8.0
+        k[200:, :, 1] = -64.0
+        k[290] = 24.0
+    for kind in ("bf16", "fp32"):
+        for new in (1, 80):
+            check_attend(torch, [300], [new], 64, 1, 2, 16, kind, True, spoil=spoil)
+
+
+def test_bounds_that_the_host_states(torch):
+    """A longer request than max_length is seen up to it; tokens beyond a table row are not; rows behind max_new are left."""
+    rng = np.random.default_rng(9)
+    mem = Memory(torch, rng, [200, 90], 64, 1, 16)
+    q, qx = as_type(torch, rng.standard_normal((6, 2, 64)), "fp32")
+    got, lse, _ = attend(mem, q, [3, 3], 2, "fp32", True, 0.2, max_length=100)
+    check_rows(mem, got, lse, qx, [(r, r // 3) for r in range(6)], 2, "fp32", float(np.float32(0.2)), lambda r, i: slice(0, 100 if i == 0 else 88 + r % 3))
+    got, lse, _ = attend(mem, q, [3, 3], 2, "fp32", False, 0.2, max_new=2)
+    check_rows(mem, got, lse, qx, [(r, r // 3) for r in (0, 1, 3, 4)], 2, "fp32", float(np.float32(0.2)), lambda r, i: slice(0, mem.lengths[i]))
+    assert (got[[2, 5]] == 77.0).all()
+    mem.stride = 13  # row 0: 13 pages of 16 = 208 tokens that the table can name; the request says more
+    got, lse, _ = attend(mem, q, [3, 3], 2, "fp32", False, 0.2, lengths=[5000, 90], tables=mem.tables[:, :13])
+    check_rows(mem, got, lse, qx, [(r, 1) for r in (3, 4, 5)], 2, "fp32", float(np.float32(0.2)), lambda r, i: slice(0, 90))
+
+
+def test_starts_that_reach_behind_the_rows_stay_inside(torch):
+    rng = np.random.default_rng(10)
+    mem = Memory(torch, rng, [64, 64], 64, 1, 16)
+    q, qx = as_type(torch, rng.standard_normal((4, 1, 64)), "bf16")
+    got, lse, _ = attend(mem, q, [2, 40], 1, "bf16", False, 0.2, rows=4, max_new=40)
+    check_rows(mem, got, lse, qx, [(r, r // 2) for r in range(4)], 1, "bf16", float(np.float32(0.2)), lambda r, i: slice(0, 64))
+    assert (got[4:] == 77.0).all()
+
+
+def test_strided_queries_and_no_lse(torch):
+    rng = np.random.default_rng(11)
+    mem = Memory(torch, rng, [77, 5], 64, 2, 16)
+    wide, wx = as_type(torch, rng.standard_normal((5, 3 * 4 * 64 + 8)), "bf16")  # a fused projection's rows
+    got, lse, _ = attend(mem, wide, [3, 2], 2, "bf16", True, 0.125, q_stride=wide.shape[1], lse=False)
+    qx = wx[:, :256].reshape(5, 4, 64)
+    assert (lse == 77.0).all()
+    _, full, _ = attend(mem, wide, [3, 2], 2, "bf16", True, 0.125, q_stride=wide.shape[1])
+    check_rows(mem, got, full, qx, [(0, 0), (1, 0), (2, 0), (3, 1), (4, 1)], 2, "bf16", 0.125, lambda r, i: slice(0, mem.lengths[i] - (3, 2)[i] + (r - 3 * i) + 1))
+
+
+@pytest.mark.parametrize("new", [1, 65])
+def test_the_same_inputs_give_the_same_bits(torch, new):
+    rng = np.random.default_rng(12)
+    mem = Memory(torch, rng, [1500, 900], 128, 2, 16)
+    q, _ = as_type(torch, rng.standard_normal((2 * new, 8, 128)), "bf16")
+    a = attend(mem, q, [new, new], 4, "bf16", True, 0.1)
+    for _ in range(3):
+        b = attend(mem, q, [new, new], 4, "bf16", True, 0.1)
+        assert np.array_equal(a[0], b[0]) and np.array_equal(a[1], b[1])
+
+
+def test_a_workspace_that_is_too_small_is_refused(torch):
+    import zvdb_amd as zv
+    rng = np.random.default_rng(13)
+    mem = Memory(torch, rng, [1500], 64, 1, 16)
+    q, _ = as_type(torch, rng.standard_normal((1, 1, 64)), "bf16")
+    size = mem.lay.attend_workspace(zv.KV_BF16, 1, 1, 1, 1, 1500)
+    ws, out, S, L, T = torch.empty(size, dtype=torch.uint8, device="cuda"), torch.empty_like(q), mem.i32([0, 1]), mem.i32([1500]), mem.i32(mem.tables)
+    for p, b in ((ws.data_ptr(), size - 1), (0, size), (ws.data_ptr() + 8, size)):
+        with pytest.raises(zv.ZvdbError) as e:
+            mem.lay.attend_dev(mem.cache.data_ptr(), q.data_ptr(), 64, zv.KV_BF16, 1, 1, S.data_ptr(), 1, 1, L.data_ptr(), T.data_ptr(), mem.stride, 1500, 0.1, True, p, b,
+                               out.data_ptr(), 0, stream(torch))
+        assert e.value.code == 1
+
+
+def test_host_memory_is_refused(torch):
+    import zvdb_amd as zv
+    lay = zv.KVLayout(head_dim=64, kv_heads=1, page_size=16, pages=1)
+    for pin in (False, True):
+        host = torch.zeros(1 << 16, dtype=torch.uint8)
+        host = host.pin_memory() if pin else host
+        dev = torch.zeros(1 << 16, dtype=torch.uint8, device="cuda")
+        at = (host.data_ptr() + 15) // 16 * 16
+        with pytest.raises(zv.ZvdbError) as e:
+            lay.read_dev(at, dev.data_ptr(), 1, dev.data_ptr(), 0, 0, stream(torch))
+        assert e.value.code == 1
+
+
+def test_a_cache_beyond_32_bits_of_bytes(torch):
+    """Pages behind 4 GiB and behind 2^31 slots' worth of bytes: the same answers as in a small cache."""
+    rng = np.random.default_rng(14)
+    import zvdb_amd as zv
+    mem = Memory(torch, rng, [300, 65], 128, 2, 16)
+    big = zv.KVLayout(head_dim=128, kv_heads=2, page_size=16, pages=(10 << 30) // mem.lay.page_bytes)
+    far = torch.empty(big.pages * big.page_bytes, dtype=torch.uint8, device="cuda")
+    move = big.pages - mem.pages
+    far[move * big.page_bytes:] = mem.cache
+    q, _ = as_type(torch, rng.standard_normal((42, 4, 128)), "bf16")
+    for new in ([1, 1], [40, 2]):
+        want = attend(mem, q, new, 2, "bf16", True, 0.1)
+        small = (mem.lay, mem.cache, mem.tables)
+        mem.lay, mem.cache, mem.tables = big, far, np.where(mem.tables < mem.pages, mem.tables + move, mem.tables).astype(np.uint32)
+        got = attend(mem, q, new, 2, "bf16", True, 0.1)
+        mem.lay, mem.cache, mem.tables = small
+        assert np.array_equal(got[0], want[0]) and np.array_equal(got[1], want[1])
+    slots = torch.tensor([move * 16 + 3, big.pages * 16 - 1], device="cuda")
+    k = torch.randn(2, 2, 128, device="cuda")
+    big.append_dev(far.data_ptr(), k.data_ptr(), 256, k.data_ptr(), 256, zv.KV_F32, 2, slots.data_ptr(), stream(torch))
+    mem.lay.append_dev(mem.cache.data_ptr(), k.data_ptr(), 256, k.data_ptr(), 256, zv.KV_F32, 2, (slots - move * 16).data_ptr(), stream(torch))
+    assert torch.equal(far[move * big.page_bytes:], mem.cache)
+    a, b = torch.empty_like(k), torch.empty_like(k)
+    big.read_dev(far.data_ptr(), slots.data_ptr(), 2, a.data_ptr(), b.data_ptr(), zv.KV_F32, stream(torch))
+    assert torch.equal(a, b) and torch.isfinite(a).all()
+
+
+# ---- attention over selected rows -------------------------------------------------------------------------------------------------
+
+def selected(mem, q, ids, counts, group, kind, scale, lengths=None):
+    torch = mem.torch
+    heads, n, k = ids.shape
+    qh = heads * group
+    out = torch.full((n + 1, qh, mem.d), 77.0, dtype=q.dtype, device="cuda")
+    lse = torch.full((n + 1, qh), 77.0, device="cuda")
+    I = torch.tensor(ids.astype(np.uint64).view(np.int64), device="cuda")
+    C = mem.i32(counts) if counts is not None else None
+    L, T = mem.i32(mem.lengths if lengths is None else lengths), mem.i32(mem.tables)
+    mem.lay.attend_selected_dev(mem.cache.data_ptr(), q.data_ptr(), qh * mem.d, kv_type(kind), qh, n, I.data_ptr(), C.data_ptr() if C is not None else 0, k,
+                                L.data_ptr(), T.data_ptr(), mem.stride, scale, out.data_ptr(), lse.data_ptr(), stream(torch))
+    torch.cuda.synchronize()
+    assert (out[n] == 77.0).all() and (lse[n] == 77.0).all()
+    return out.double().cpu().numpy(), lse.double().cpu().numpy()
+
+
+def check_selected(mem, got, lse, qx, ids, counts, group, kind, scale, there=None):
+    heads, n, k = ids.shape
+    for i in range(n):
+        for h in range(heads * group):
+            m = k if counts is None else min(int(counts[h // group, i]), k)
+            see = [int(t) for t in ids[h // group, i, :m] if int(t) < mem.lengths[i] and (there is None or there(i, int(t)))]
+            kh, vh = mem.k[mem.rows_of(i)][see, h // group], mem.v[mem.rows_of(i)][see, h // group]
+            with np.errstate(invalid="ignore"):
+                o, l, bo, bl = ref.attend_row(qx[i, h], kh, vh, scale, kind)
+            if np.isnan(kh).any():
+                assert np.isnan(got[i, h]).all() and np.isnan(lse[i, h])
+                continue
+            bad = np.isnan(vh).any(0)
+            assert np.array_equal(np.isnan(got[i, h]), bad), (i, h)
+            assert (np.abs(got[i, h] - o)[~bad] <= bo[~bad]).all(), (i, h)
+            assert lse[i, h] == l or abs(lse[i, h] - l) <= bl, (i, h, lse[i, h], l)
+
+
+@pytest.mark.parametrize("kind", ["bf16", "fp32"])
+@pytest.mark.parametrize("d,heads,group,page,k", [(64, 2, 1, 16, 10), (64, 1, 4, 32, 1), (96, 2, 3, 16, 33), (128, 2, 4, 64, 100), (128, 1, 20, 16, 129), (256, 1, 2, 16, 40),
+                                                  (64, 1, 2, 16, 1100)])
+def test_selected_rows(torch, kind, d, heads, group, page, k):
+    rng = np.random.default_rng(d + k)
+    lengths = [300, 1, 77, 1500 if k > 1000 else 40]
+    mem = Memory(torch, rng, lengths, d, heads, page)
+    n = len(lengths)
+    ids = rng.integers(0, 1500, (heads, n, k)).astype(np.uint64)          # many are behind the request's tokens; some twice
+    for h in range(heads):
+        for i in range(n):
+            ids[h, i, ::2] = rng.integers(0, lengths[i], len(ids[h, i, ::2]))
+    ids[:, :, k // 2] = 2**64 - 1
+    ids[:, 2, -1] = 2**32 + 5                                              # not token 5
+    counts = rng.integers(0, k + 1, (heads, n))
+    counts[0, 0], counts[-1, 1], counts[0, 2] = k, 0, k + 7                # more than k is k
+    q, qx = as_type(torch, rng.standard_normal((n, heads * group, d)), kind)
+    for c in (counts, None):
+        got, lse = selected(mem, q, ids, c, group, kind, 0.3)
+        check_selected(mem, got, lse, qx, ids, c, group, kind, float(np.float32(0.3)))
+
+
+def test_selected_rows_of_hidden_pages_and_nan(torch):
+    rng = np.random.default_rng(21)
+
+    def spoil(mem, k, v):
+        v[20, 0, 40] = np.nan
+        k[150, 1, 3] = np.nan
+    mem = Memory(torch, rng, [100, 90], 64, 2, 16, spoil=spoil)
+    mem.tables[0, 4] = mem.pages
+    ids = np.stack([np.stack([rng.permutation(90)[:40] for _ in range(2)]) for _ in range(2)]).astype(np.uint64)
+    ids[0, 0, 3], ids[1, 0, 5] = 20, 20
+    ids[0, 1, 0], ids[1, 1, 0] = 50, 50
+    q, qx = as_type(torch, rng.standard_normal((2, 4, 64)), "bf16")
+    got, lse = selected(mem, q, ids, None, 2, "bf16", 0.3)
+    check_selected(mem, got, lse, qx, ids, None, 2, "bf16", float(np.float32(0.3)), there=lambda i, t: not (i == 0 and t // 16 == 4))
+
+
+def test_selecting_every_row_is_attending_to_all(torch):
+    rng = np.random.default_rng(22)
+    mem = Memory(torch, rng, [130, 64], 128, 2, 16)
+    q, qx = as_type(torch, rng.standard_normal((2, 8, 128)), "fp32")
+    ids = np.tile(np.arange(130, dtype=np.uint64), (2, 2, 1))
+    got, lse = selected(mem, q, ids, None, 4, "fp32", 0.1)
+    want, wl, _ = attend(mem, q, [1, 1], 4, "fp32", False, 0.1)
+    for i in range(2):
+        for h in range(8):
+            _, _, bo, bl = ref.attend_row(qx[i, h], mem.k[mem.rows_of(i)][:, h // 4], mem.v[mem.rows_of(i)][:, h // 4], float(np.float32(0.1)), "fp32")
+            assert (np.abs(got[i, h] - want[i, h]) <= 2 * bo).all() and abs(lse[i, h] - wl[i, h]) <= 2 * bl

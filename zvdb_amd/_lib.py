@@ -37,6 +37,13 @@ class CertInfo(C.Structure):
                 ("bound_checked", C.c_uint32), ("bound_violations", C.c_uint32)]
 
 
+class KvLayoutStruct(C.Structure):
+    _fields_ = [("abi_version", C.c_uint32), ("head_dim", C.c_uint32), ("kv_heads", C.c_uint32), ("page_size", C.c_uint32),
+                ("pages", C.c_uint64)]
+
+
+KV_F32, KV_BF16 = 0, 1
+KV_PLANNED, KV_OUT_OF_PAGES, KV_TABLE_TOO_SHORT, KV_SLOTS_TOO_FEW = range(4)
 OPT_CERTIFY, OPT_CERT_MIN_LEVEL, OPT_CERT_FORCE_REPAIR, OPT_EF_SEARCH_WIDTH = 1, 2, 3, 4
 
 
@@ -102,6 +109,15 @@ HIP_SYMBOLS = [
     ("zvdb_hip_search_graph_sharded_dev", _i32, [_vp, _vp, _vp, _u32, _u32, _u32, _u32, _u64, _u64, _vp, _u64, _vp, _vp, _vp, _vp, _vp]),
     ("zvdb_hip_timing_enable", _i32, [_vp, _i32]),
     ("zvdb_hip_timing_read", _i32, [_vp, C.POINTER(C.c_double), _u32p]),
+    ("zvdb_hip_kv_page_bytes", _i32, [C.POINTER(KvLayoutStruct), _u64p]),
+    ("zvdb_hip_kv_plan_dev", _i32, [C.POINTER(KvLayoutStruct), _vp, _vp, _u32, _vp, _u32, _vp, _vp, _u32, _vp, _vp, _u64, _vp, _vp, _vp, _vp]),
+    ("zvdb_hip_kv_append_dev", _i32, [C.POINTER(KvLayoutStruct), _vp, _vp, _u64, _vp, _u64, _u32, _u32, _vp, _vp]),
+    ("zvdb_hip_kv_read_dev", _i32, [C.POINTER(KvLayoutStruct), _vp, _vp, _u32, _vp, _vp, _u32, _vp]),
+    ("zvdb_hip_kv_attend_workspace", _i32, [C.POINTER(KvLayoutStruct), _u32, _u32, _u32, _u32, _u32, _u32, _u64p]),
+    ("zvdb_hip_kv_attend_dev", _i32, [C.POINTER(KvLayoutStruct), _vp, _vp, _u64, _u32, _u32, _u32, _vp, _u32, _u32, _vp, _vp, _u32, _u32,
+                                      C.c_float, _u32, _vp, _u64, _vp, _vp, _vp]),
+    ("zvdb_hip_kv_attend_selected_dev", _i32, [C.POINTER(KvLayoutStruct), _vp, _vp, _u64, _u32, _u32, _u32, _vp, _vp, _u32, _vp, _vp, _u32,
+                                               C.c_float, _vp, _vp, _vp]),
 ]
 
 HOST_SYMBOLS = [

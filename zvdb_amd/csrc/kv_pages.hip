@@ -1,0 +1,405 @@
+// kv_pages.hip -- the 4-bit key/value cache's pages: planning (block tables, slot map), writing rows, reading them back.
+//
+// All three are bound by latency when a decode step calls them and by HBM when a prompt does; none has arithmetic worth counting.
+#include "kv_cache.h"
+
+#include <algorithm>
+
+namespace zvdb {
+
+int kv_check_layout(const zvdb_hip_kv_layout *l, KvGeom *g) {
+    KV_ARG(l, "null layout");
+    KV_ARG(l->abi_version == ZVDB_HIP_ABI_VERSION, "kv layout: ABI version %u, library %u", l->abi_version, (unsigned)ZVDB_HIP_ABI_VERSION);
+    KV_ARG(l->head_dim >= 8 && l->head_dim <= 256 && l->head_dim % 8 == 0, "kv layout: head_dim %u (a multiple of 8 up to 256)", l->head_dim);
+    KV_ARG(l->kv_heads >= 1 && l->kv_heads <= 1024, "kv layout: kv_heads %u (1 .. 1024)", l->kv_heads);
+    KV_ARG(l->page_size >= 16 && l->page_size <= 256 && (l->page_size & (l->page_size - 1)) == 0, "kv layout: page_size %u (16, 32, 64, 128 or 256)", l->page_size);
+    KV_ARG(l->pages >= 1 && l->pages < 0x7FFFFFFFu, "kv layout: %llu pages (1 .. 2^31 - 2)", (unsigned long long)l->pages);
+    g->head_bytes = (uint32_t)kv_head_bytes(l);
+    g->page_bytes = (uint64_t)g->head_bytes * l->kv_heads;
+    g->pages = (uint32_t)l->pages;
+    g->heads = l->kv_heads;
+    g->dim = l->head_dim;
+    g->page_size = l->page_size;
+    g->page_shift = (uint32_t)__builtin_ctz(l->page_size);
+    return ZVDB_OK;
+}
+
+int KvDevice::enter(const void *p, hipStream_t s) {
+    int n = 0;
+    if (hipGetDeviceCount(&n) != hipSuccess || n == 0) {
+        (void)hipGetLastError();
+        set_error("no HIP device");
+        return ZVDB_ERR_NO_DEVICE;
+    }
+    hipPointerAttribute_t at;
+    if (hipPointerGetAttributes(&at, p) != hipSuccess || (at.type != hipMemoryTypeDevice && at.type != hipMemoryTypeManaged) || at.device < 0 || at.device >= n) {
+        (void)hipGetLastError();
+        set_error("a kv call needs device memory");
+        return ZVDB_ERR_INVALID;
+    }
+    if (s) {
+        hipDevice_t d = 0;
+        ZV_HIP(hipStreamGetDevice(s, &d));
+        KV_ARG(d == at.device, "the stream is of device %d, the memory of device %d", (int)d, at.device);
+    }
+    int cur = 0;
+    ZV_HIP(hipGetDevice(&cur));
+    if (cur != at.device) {
+        ZV_HIP(hipSetDevice(at.device));
+        prev_ = cur;
+    }
+    ZV_HIP(hipDeviceGetAttribute(&cus_, hipDeviceAttributeMultiprocessorCount, at.device));
+    return ZVDB_OK;
+}
+
+// ---- plan ---------------------------------------------------------------------------------------------------------------
+
+struct KvPlanArgs {
+    const uint32_t *lengths, *fresh, *ring;
+    const uint64_t *cursor;
+    uint32_t *tables, *starts, *out_lengths, *status;
+    uint64_t *slots, *out_cursor;
+    uint64_t slot_cap;
+    uint32_t n, ring_size, table_stride, pages, page_shift;
+};
+
+constexpr uint32_t kPlanMax = 16384;  // requests of a call: two prefix sums of them lie in LDS
+
+// last i with first[i] <= x, in first[0 .. n] (first[0] = 0 <= x < first[n])
+__device__ inline uint32_t kv_owner(const uint32_t *first, uint32_t n, uint32_t x) {
+    uint32_t lo = 0, hi = n;  // first[lo] <= x < first[hi]
+    while (hi - lo > 1) {
+        const uint32_t mid = (lo + hi) >> 1;
+        if (first[mid] <= x) lo = mid;
+        else hi = mid;
+    }
+    return lo;
+}
+
+// Every block forms the two prefix sums of the whole batch (tokens and pages; 8 n bytes that stay in L2) and fills its share of
+// the slots and of the new table entries: one launch, no block waits for another, and nothing that a block reads is written by
+// one (a partly filled page's table entry is an older call's; new pages are read from the ring).  Bound by latency up to some
+// thousand tokens, by the 8-byte slot stores beyond.
+__global__ __launch_bounds__(1024) void k_kv_plan(const KvPlanArgs a) {
+    extern __shared__ uint32_t lds[];
+    uint32_t *const tok = lds, *const pag = lds + a.n + 1;  // [n + 1] each
+    __shared__ uint64_t wt[16], wp[16];
+    __shared__ uint32_t bad;
+    const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, nt = blockDim.x;
+    const uint32_t per = (a.n + nt - 1) / nt, i0 = min(tid * per, a.n), i1 = min(i0 + per, a.n);
+    const uint32_t mask = (1u << a.page_shift) - 1;
+    if (tid == 0) bad = 0;
+    __syncthreads();
+    uint64_t st = 0, sp = 0;
+    for (uint32_t i = i0; i < i1; ++i) {
+        const uint64_t c = a.lengths[i], e = c + a.fresh[i];
+        const uint64_t have = (c + mask) >> a.page_shift, want = (e + mask) >> a.page_shift;
+        if (want > a.table_stride || e > 0x7FFFFFFFull) bad = 1;  // (every writer writes the same)
+        st += e - c;
+        sp += want - have;
+    }
+    uint64_t it = st, ip = sp;  // inclusive scan over the block's threads
+    for (int d = 1; d < 64; d <<= 1) {
+        const uint64_t t = __shfl_up(it, d), p = __shfl_up(ip, d);
+        if (lane >= (uint32_t)d) { it += t; ip += p; }
+    }
+    if (lane == 63) { wt[wave] = it; wp[wave] = ip; }
+    __syncthreads();
+    uint64_t bt = 0, bp = 0, tt = 0, tp = 0;
+    for (uint32_t w = 0; w < nt / 64; ++w) {
+        if (w < wave) { bt += wt[w]; bp += wp[w]; }
+        tt += wt[w];
+        tp += wp[w];
+    }
+    const uint64_t taken = a.cursor[0], given = a.cursor[1];
+    const uint64_t left = given > taken ? min(given - taken, (uint64_t)a.ring_size) : 0;
+    const uint32_t code = bad ? ZVDB_KV_TABLE_TOO_SHORT : tt > a.slot_cap ? ZVDB_KV_SLOTS_TOO_FEW : tp > left ? ZVDB_KV_OUT_OF_PAGES : ZVDB_KV_PLANNED;
+    const bool ok = code == ZVDB_KV_PLANNED;  // then both totals fit 32 bits: slot_cap and the ring do
+    if (ok) {
+        uint32_t xt = (uint32_t)(bt + it - st), xp = (uint32_t)(bp + ip - sp);
+        for (uint32_t i = i0; i < i1; ++i) {
+            tok[i] = xt;
+            pag[i] = xp;
+            const uint32_t c = a.lengths[i], e = c + a.fresh[i];
+            xt += e - c;
+            xp += ((e + mask) >> a.page_shift) - ((c + mask) >> a.page_shift);
+        }
+        if (tid == 0) { tok[a.n] = (uint32_t)tt; pag[a.n] = (uint32_t)tp; }
+    }
+    __syncthreads();
+    if (blockIdx.x == 0) {
+        for (uint32_t i = tid; i <= a.n; i += nt) a.starts[i] = ok ? tok[i] : 0;
+        for (uint32_t i = tid; i < a.n; i += nt) a.out_lengths[i] = a.lengths[i] + (ok ? a.fresh[i] : 0);
+        if (tid == 0) {
+            a.out_cursor[0] = taken + (ok ? tp : 0);
+            a.out_cursor[1] = given;
+            a.status[0] = code;
+            a.status[1] = (uint32_t)min(tp, (uint64_t)0x7FFFFFFF);
+            a.status[2] = (uint32_t)min(tt, (uint64_t)0x7FFFFFFF);
+            a.status[3] = 0;
+        }
+    }
+    const uint32_t base = (uint32_t)(taken % a.ring_size);
+    auto fresh_page = [&](uint32_t x) {  // the x-th page the batch takes; x < ring_size
+        const uint64_t r = (uint64_t)base + x;
+        return a.ring[r >= a.ring_size ? r - a.ring_size : r];
+    };
+    const uint64_t step = (uint64_t)gridDim.x * nt, at = (uint64_t)blockIdx.x * nt + tid;
+    for (uint64_t t = at; t < a.slot_cap; t += step) {
+        uint64_t slot = ~0ull;
+        if (ok && t < tt) {
+            const uint32_t i = kv_owner(tok, a.n, (uint32_t)t), c = a.lengths[i], pos = c + ((uint32_t)t - tok[i]);
+            const uint32_t have = (c + mask) >> a.page_shift, p = pos >> a.page_shift;
+            const uint32_t page = p < have ? a.tables[(uint64_t)i * a.table_stride + p] : fresh_page(pag[i] + p - have);
+            if (page < a.pages) slot = ((uint64_t)page << a.page_shift) | (pos & mask);
+        }
+        a.slots[t] = slot;
+    }
+    if (!ok) return;
+    for (uint64_t x = at; x < tp; x += step) {
+        const uint32_t i = kv_owner(pag, a.n, (uint32_t)x), have = (a.lengths[i] + mask) >> a.page_shift;
+        a.tables[(uint64_t)i * a.table_stride + have + ((uint32_t)x - pag[i])] = fresh_page((uint32_t)x);
+    }
+}
+
+// ---- append -------------------------------------------------------------------------------------------------------------
+
+template <class T>
+__device__ inline void kv_load8(const T *p, float *x) {
+    if constexpr (sizeof(T) == 2) {
+        const uint4 u = *reinterpret_cast<const uint4 *>(p);
+        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            x[2 * i] = __uint_as_float(w[i] << 16);
+            x[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+        }
+    } else {
+        const float4 u = *reinterpret_cast<const float4 *>(p), v = *reinterpret_cast<const float4 *>(p + 4);
+        x[0] = u.x; x[1] = u.y; x[2] = u.z; x[3] = u.w;
+        x[4] = v.x; x[5] = v.y; x[6] = v.z; x[7] = v.w;
+    }
+}
+
+// One lane takes 8 elements of a row, four lanes a block of 32.  The block's scale is the power of two at or under its largest
+// magnitude over E2M1's 4 -- the next one from 7/4 of it on, where 6 would be nearer than 8 and the largest element would lose an
+// eighth and more of itself.  A power of two divides exactly, so the code is the nearest of x / scale, ties to even (bf16 rows
+// meet ties often: 8 significant bits over a grid of 3), saturating at 6.  Lanes of one wave hold consecutive tokens of ONE head:
+// the four tokens of a V group are written by neighbouring lanes into the same 16 pieces.
+template <class T, int NB>
+__global__ __launch_bounds__(256) void k_kv_append(uint8_t *cache, const KvGeom g, const T *k, uint64_t k_stride, const T *v, uint64_t v_stride,
+                                                   const uint64_t *slots, uint32_t n) {
+    constexpr uint32_t L = 4 * NB;  // lanes of a row
+    const uint32_t c8 = threadIdx.x % L, head = blockIdx.y;
+    const uint64_t i = (uint64_t)blockIdx.x * (256 / L) + threadIdx.x / L;
+    if (i >= n) return;  // (whole rows leave: the four lanes of a block stay together)
+    const uint64_t slot = slots[i];
+    if (slot >= (uint64_t)g.pages << g.page_shift) return;
+    const bool value = blockIdx.z;
+    const T *src = (value ? v + i * v_stride : k + i * k_stride) + (uint64_t)head * g.dim + c8 * 8;
+    float x[8] = {};
+    if (c8 * 8 < g.dim) kv_load8(src, x);
+    uint32_t top = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) top = max(top, __float_as_uint(x[j]) & 0x7FFFFFFFu);
+    top = max(top, (uint32_t)__shfl_xor((int)top, 1));
+    top = max(top, (uint32_t)__shfl_xor((int)top, 2));
+    const int e = (int)((top + 0x200000u) >> 23) - 2;
+    uint32_t b = (uint32_t)min(max(e, (int)kKvScaleMin), (int)kKvScaleMax), code = 0;
+    if (top >= 0x7F800000u) {
+        b = kKvScaleNaN;
+    } else {
+        const float s = __uint_as_float(b << 23);
+        code = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(code, x[0], x[1], s, 0);
+        code = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(code, x[2], x[3], s, 1);
+        code = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(code, x[4], x[5], s, 2);
+        code = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(code, x[6], x[7], s, 3);
+    }
+    const uint32_t t = (uint32_t)slot & (g.page_size - 1), half = g.page_size * 16 * NB;
+    uint8_t *const at = cache + (slot >> g.page_shift) * g.page_bytes + (uint64_t)head * g.head_bytes;
+    uint8_t *const scales = at + 2 * half;
+    if (!value) {
+        *reinterpret_cast<uint32_t *>(at + t * (16 * NB) + c8 * 4) = code;
+        if (c8 % 4 == 0) scales[t * NB + c8 / 4] = (uint8_t)b;
+    } else {
+        uint8_t *const w = at + half;
+        if constexpr (NB == 2) {
+            *reinterpret_cast<uint16_t *>(w + kv_v_offset<NB>(t, 2 * c8)) = (uint16_t)code;
+            *reinterpret_cast<uint16_t *>(w + kv_v_offset<NB>(t, 2 * c8 + 1)) = (uint16_t)(code >> 16);
+        } else if constexpr (NB == 4) {
+            *reinterpret_cast<uint32_t *>(w + kv_v_offset<NB>(t, c8)) = code;
+        } else {
+            *reinterpret_cast<uint32_t *>(w + kv_v_offset<NB>(t, c8 / 2) + (c8 % 2) * 4) = code;
+        }
+        if (c8 % 4 == 0) scales[g.page_size * NB + (t >> 2) * (4 * NB) + c8 + (t & 3)] = (uint8_t)b;
+    }
+}
+
+// ---- read ---------------------------------------------------------------------------------------------------------------
+
+template <class T>
+__device__ inline void kv_store8(T *p, const float *x) {
+    if constexpr (sizeof(T) == 2) {  // a code times a power of two is a bf16 number: nothing is rounded
+        uint32_t w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = (__float_as_uint(x[2 * i]) >> 16) | (__float_as_uint(x[2 * i + 1]) & 0xFFFF0000u);
+        *reinterpret_cast<uint4 *>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+    } else {
+        *reinterpret_cast<float4 *>(p) = make_float4(x[0], x[1], x[2], x[3]);
+        *reinterpret_cast<float4 *>(p + 4) = make_float4(x[4], x[5], x[6], x[7]);
+    }
+}
+
+// The append's lanes the other way round; a slot that is not in the cache reads as zeros.
+template <class T, int NB>
+__global__ __launch_bounds__(256) void k_kv_read(const uint8_t *cache, const KvGeom g, const uint64_t *slots, uint32_t n, T *k, T *v) {
+    constexpr uint32_t L = 4 * NB;
+    const uint32_t c8 = threadIdx.x % L, head = blockIdx.y;
+    const uint64_t i = (uint64_t)blockIdx.x * (256 / L) + threadIdx.x / L;
+    const bool value = k == nullptr || blockIdx.z;
+    T *const dst = value ? v : k;
+    if (i >= n || c8 * 8 >= g.dim) return;
+    const uint64_t slot = slots[i];
+    float x[8] = {};
+    if (slot < (uint64_t)g.pages << g.page_shift) {
+        const uint32_t t = (uint32_t)slot & (g.page_size - 1), half = g.page_size * 16 * NB;
+        const uint8_t *const at = cache + (slot >> g.page_shift) * g.page_bytes + (uint64_t)head * g.head_bytes;
+        const uint8_t *const scales = at + 2 * half;
+        uint32_t code, b;
+        if (!value) {
+            code = *reinterpret_cast<const uint32_t *>(at + t * (16 * NB) + c8 * 4);
+            b = scales[t * NB + c8 / 4];
+        } else {
+            const uint8_t *const w = at + half;
+            if constexpr (NB == 2)
+                code = *reinterpret_cast<const uint16_t *>(w + kv_v_offset<NB>(t, 2 * c8)) |
+                       (uint32_t)*reinterpret_cast<const uint16_t *>(w + kv_v_offset<NB>(t, 2 * c8 + 1)) << 16;
+            else if constexpr (NB == 4)
+                code = *reinterpret_cast<const uint32_t *>(w + kv_v_offset<NB>(t, c8));
+            else
+                code = *reinterpret_cast<const uint32_t *>(w + kv_v_offset<NB>(t, c8 / 2) + (c8 % 2) * 4);
+            b = scales[g.page_size * NB + (t >> 2) * (4 * NB) + (c8 & ~3u) + (t & 3)];
+        }
+        const float s = __uint_as_float(b << 23);
+        const bf16x2 y[4] = {__builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(code, s, 0), __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(code, s, 1),
+                             __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(code, s, 2), __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(code, s, 3)};
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] = b == kKvScaleNaN ? __uint_as_float(0x7FC00000u) : (float)y[j / 2][j % 2];
+    }
+    kv_store8(dst + ((i * g.heads + head) * g.dim + c8 * 8), x);
+}
+
+template <class T>
+static void launch_append(uint8_t *cache, const KvGeom &g, const void *k, uint64_t ks, const void *v, uint64_t vs, const uint64_t *slots, uint32_t n, hipStream_t s) {
+    const T *kk = static_cast<const T *>(k), *vv = static_cast<const T *>(v);
+    const uint32_t w = kv_width(g.dim), rows = 256 / (w / 8);
+    const dim3 grid((n + rows - 1) / rows, g.heads, 2);
+    if (w == 64) hipLaunchKernelGGL((k_kv_append<T, 2>), grid, dim3(256), 0, s, cache, g, kk, ks, vv, vs, slots, n);
+    else if (w == 128) hipLaunchKernelGGL((k_kv_append<T, 4>), grid, dim3(256), 0, s, cache, g, kk, ks, vv, vs, slots, n);
+    else hipLaunchKernelGGL((k_kv_append<T, 8>), grid, dim3(256), 0, s, cache, g, kk, ks, vv, vs, slots, n);
+}
+
+template <class T>
+static void launch_read(const uint8_t *cache, const KvGeom &g, const uint64_t *slots, uint32_t n, void *k, void *v, hipStream_t s) {
+    T *kk = static_cast<T *>(k), *vv = static_cast<T *>(v);
+    const uint32_t w = kv_width(g.dim), rows = 256 / (w / 8);
+    const dim3 grid((n + rows - 1) / rows, g.heads, k && v ? 2 : 1);
+    if (w == 64) hipLaunchKernelGGL((k_kv_read<T, 2>), grid, dim3(256), 0, s, cache, g, slots, n, kk, vv);
+    else if (w == 128) hipLaunchKernelGGL((k_kv_read<T, 4>), grid, dim3(256), 0, s, cache, g, slots, n, kk, vv);
+    else hipLaunchKernelGGL((k_kv_read<T, 8>), grid, dim3(256), 0, s, cache, g, slots, n, kk, vv);
+}
+
+}  // namespace zvdb
+
+using namespace zvdb;
+
+extern "C" {
+
+int zvdb_hip_kv_page_bytes(const zvdb_hip_kv_layout *layout, uint64_t *out_bytes) {
+    KvGeom g;
+    ZV_CHECK(kv_check_layout(layout, &g));
+    KV_ARG(out_bytes, "null argument");
+    *out_bytes = g.page_bytes;
+    return ZVDB_OK;
+}
+
+int zvdb_hip_kv_plan_dev(const zvdb_hip_kv_layout *layout, const void *d_lengths, const void *d_new, uint32_t n, const void *d_ring,
+                         uint32_t ring_size, const void *d_cursor, void *d_tables, uint32_t table_stride, void *d_starts, void *d_slots,
+                         uint64_t slot_cap, void *d_out_lengths, void *d_out_cursor, void *d_status, void *stream) {
+    KvGeom g;
+    ZV_CHECK(kv_check_layout(layout, &g));
+    KV_ARG(d_cursor && d_ring && d_starts && d_out_cursor && d_status, "null argument");
+    KV_ARG(n == 0 || (d_lengths && d_new && d_tables && d_out_lengths), "null argument");
+    KV_ARG(slot_cap == 0 || d_slots, "null argument");
+    KV_ARG(n <= kPlanMax, "kv_plan: %u requests (at most %u)", n, kPlanMax);
+    KV_ARG(ring_size >= 1 && ring_size < 0x7FFFFFFFu, "kv_plan: a ring of %u pages", ring_size);
+    KV_ARG(table_stride >= 1 && table_stride < 0x7FFFFFFFu, "kv_plan: table_stride %u", table_stride);
+    KV_ARG(slot_cap < 0x7FFFFFFFu, "kv_plan: %llu slots (below 2^31 - 1)", (unsigned long long)slot_cap);
+    KV_ARG(kv_aligned(d_cursor, 8) && kv_aligned(d_out_cursor, 8) && kv_aligned(d_slots, 8), "kv_plan: a 64-bit array is not 8-byte aligned");
+    KV_ARG(d_out_cursor != d_cursor && (n == 0 || (d_out_lengths != d_lengths && d_out_lengths != d_new)), "kv_plan: an output is an input (every block reads the inputs)");
+    const hipStream_t s = static_cast<hipStream_t>(stream);
+    KvDevice dev;
+    ZV_CHECK(dev.enter(d_status, s));
+    KvPlanArgs a;
+    a.lengths = static_cast<const uint32_t *>(d_lengths);
+    a.fresh = static_cast<const uint32_t *>(d_new);
+    a.ring = static_cast<const uint32_t *>(d_ring);
+    a.cursor = static_cast<const uint64_t *>(d_cursor);
+    a.tables = static_cast<uint32_t *>(d_tables);
+    a.starts = static_cast<uint32_t *>(d_starts);
+    a.out_lengths = static_cast<uint32_t *>(d_out_lengths);
+    a.status = static_cast<uint32_t *>(d_status);
+    a.slots = static_cast<uint64_t *>(d_slots);
+    a.out_cursor = static_cast<uint64_t *>(d_out_cursor);
+    a.slot_cap = slot_cap;
+    a.n = n; a.ring_size = ring_size; a.table_stride = table_stride; a.pages = g.pages; a.page_shift = g.page_shift;
+    const uint32_t threads = n > 1024 || slot_cap > 4096 ? 1024 : 256;
+    const uint32_t lds = (2 * n + 2) * 4;
+    // (a table entry is one 16th of a token's work at most: the slots set the grid)
+    const uint32_t blocks = (uint32_t)std::min<uint64_t>(std::max<uint64_t>((std::max<uint64_t>(slot_cap, n) + threads * 4 - 1) / (threads * 4), 1), 2 * (uint64_t)dev.cus());
+    if (lds > 64 * 1024 - 512) ZV_HIP(hipFuncSetAttribute(reinterpret_cast<const void *>(k_kv_plan), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
+    hipLaunchKernelGGL(k_kv_plan, dim3(blocks), dim3(threads), lds, s, a);
+    ZV_HIP(hipGetLastError());
+    return ZVDB_OK;
+}
+
+int zvdb_hip_kv_append_dev(const zvdb_hip_kv_layout *layout, void *d_cache, const void *d_k, uint64_t k_stride, const void *d_v, uint64_t v_stride,
+                           uint32_t type, uint32_t n, const void *d_slots, void *stream) {
+    KvGeom g;
+    ZV_CHECK(kv_check_layout(layout, &g));
+    KV_ARG(type == ZVDB_KV_F32 || type == ZVDB_KV_BF16, "kv_append: type %u", type);
+    if (n == 0) return ZVDB_OK;
+    KV_ARG(d_cache && d_k && d_v && d_slots, "null argument");
+    KV_ARG(kv_aligned(d_cache, 16) && kv_aligned(d_k, 16) && kv_aligned(d_v, 16) && kv_aligned(d_slots, 8), "kv_append: cache, k and v need 16-byte alignment, slots 8");
+    const uint64_t row = (uint64_t)g.heads * g.dim;
+    KV_ARG(k_stride >= row && v_stride >= row && k_stride % 8 == 0 && v_stride % 8 == 0, "kv_append: a token's stride is at least kv_heads * head_dim = %llu and a multiple of 8", (unsigned long long)row);
+    const hipStream_t s = static_cast<hipStream_t>(stream);
+    KvDevice dev;
+    ZV_CHECK(dev.enter(d_cache, s));
+    uint8_t *c = static_cast<uint8_t *>(d_cache);
+    const uint64_t *slots = static_cast<const uint64_t *>(d_slots);
+    if (type == ZVDB_KV_F32) launch_append<float>(c, g, d_k, k_stride, d_v, v_stride, slots, n, s);
+    else launch_append<uint16_t>(c, g, d_k, k_stride, d_v, v_stride, slots, n, s);
+    ZV_HIP(hipGetLastError());
+    return ZVDB_OK;
+}
+
+int zvdb_hip_kv_read_dev(const zvdb_hip_kv_layout *layout, const void *d_cache, const void *d_slots, uint32_t n, void *d_k, void *d_v, uint32_t type, void *stream) {
+    KvGeom g;
+    ZV_CHECK(kv_check_layout(layout, &g));
+    KV_ARG(type == ZVDB_KV_F32 || type == ZVDB_KV_BF16, "kv_read: type %u", type);
+    if (n == 0 || (!d_k && !d_v)) return ZVDB_OK;
+    KV_ARG(d_cache && d_slots, "null argument");
+    KV_ARG(kv_aligned(d_cache, 16) && kv_aligned(d_k, 16) && kv_aligned(d_v, 16) && kv_aligned(d_slots, 8), "kv_read: cache, k and v need 16-byte alignment, slots 8");
+    const hipStream_t s = static_cast<hipStream_t>(stream);
+    KvDevice dev;
+    ZV_CHECK(dev.enter(d_cache, s));
+    const uint8_t *c = static_cast<const uint8_t *>(d_cache);
+    const uint64_t *slots = static_cast<const uint64_t *>(d_slots);
+    if (type == ZVDB_KV_F32) launch_read<float>(c, g, slots, n, d_k, d_v, s);
+    else launch_read<uint16_t>(c, g, slots, n, d_k, d_v, s);
+    ZV_HIP(hipGetLastError());
+    return ZVDB_OK;
+}
+
+}  // extern "C"
