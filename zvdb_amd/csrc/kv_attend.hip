@@ -41,6 +41,8 @@ struct KvAttendArgs {
     bool causal;
 };
 
+// Row tiles of a wave when a prompt gives every wave its own: as many as its registers hold beside two chunks of raw rows, with two waves on a SIMD
+constexpr int wide_tiles(int nb, int terms) { return terms == 1 && nb <= 4 ? 3 : 1; }
 constexpr float kSlack = 8.0f;
 constexpr float kNone = -FLT_MAX;  // maximum of a row that has seen nothing: exp2(-inf - kNone) = 0, never NaN
 constexpr float kLn2 = 0.693147180559945309f;
@@ -142,11 +144,10 @@ struct KvRows {
         }
     }
 
-    // `seen(tile of tokens, i)`: whether this lane's row of row tile t sees token 4 g + i of it; asked only where MASK.
-    // `token(i, j)`: the index that nan_at counts of V token j of token tile i.
-    template <bool MASK, class Seen, class Token>
-    __device__ void step(const KvRaw<NB> &raw, float scale_log2, Seen seen, Token token) {
-        const uint32_t g = (threadIdx.x & 63) >> 4;
+    // `seen(t, i, j)`: whether this lane's row of row tile t sees token 4 g + j of token tile i; asked only where `mask` (uniform).
+    // `token(i, j)`: the index that nan_at counts of that token.
+    template <class Seen, class Token>
+    __device__ void step(const KvRaw<NB> &raw, float scale_log2, bool mask, Seen seen, Token token) {
         // V's scales; a NaN block counts as 0 here and is entered in nan_at, so that rows that do not see its token stay whole
         float vs[8];
 #pragma unroll
@@ -178,7 +179,7 @@ struct KvRows {
         bf16x8 p[NT][TERMS];
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
-            if constexpr (MASK) {
+            if (mask) {
 #pragma unroll
                 for (int j = 0; j < 8; ++j)
                     if (!seen(t, j / 4, j % 4)) s[t][j / 4][j % 4] = -INFINITY;
@@ -202,7 +203,6 @@ struct KvRows {
             }
             split_bf16<TERMS>(x, p[t]);
         }
-        (void)g;
         // byte b of a piece holds columns 2 b and 2 b + 1 of one token: widen 8 tokens, then sort the pairs by column
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
@@ -337,7 +337,7 @@ __device__ inline void join_waves(KvRows<NB, 1, TERMS> &r) {
 // walks the same tokens.  Blocks are numbered head first, so that (with 8 heads) an XCD's L2 keeps the pages of its own heads,
 // and row tiles last to first, so that the causal ones with most tokens start first.
 template <int NB, int NT, int TERMS, bool WIDE>
-__global__ __launch_bounds__(256) void k_kv_attend(const KvAttendArgs a) {
+__global__ __launch_bounds__(256, NB == 8 && TERMS == 3 ? 1 : WIDE || NB == 8 || TERMS == 3 ? 2 : 4) void k_kv_attend(const KvAttendArgs a) {
     static_assert(WIDE || NT == 1, "waves that share rows hold one tile");
     const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4;
     uint32_t b = blockIdx.x;
@@ -396,35 +396,37 @@ __global__ __launch_bounds__(256) void k_kv_attend(const KvAttendArgs a) {
         const uint8_t *heads = a.cache + (uint64_t)head * a.g.head_bytes;
         const uint32_t chunks = (t1 - t0 + 31) >> 5;
         auto page_of = [&](uint32_t t) { return table[min(t >> a.g.page_shift, last_page)]; };
+        // what a lane adds to a tile's place: the rest of an address is uniform
+        const uint32_t key_at = (lane & 15) * (16 * NB) + g * (4 * NB), key_scale_at = (lane & 15) * NB, val_at = g * (64 * NB) + (lane & 15) * (4 * NB),
+                       val_scale_at = g * (4 * NB) + v_block<NB>(lane & 15) * 4;
         auto load = [&](KvRaw<NB> &raw, uint32_t t, const uint32_t *page) {
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
                 const uint8_t *p = heads + (uint64_t)(page[x] < a.g.pages ? page[x] : 0) * a.g.page_bytes;
-                const uint32_t in = (t + 16 * x) & mask, tok = in + (lane & 15), quad = (in >> 2) + g;
-                load_words<NB>(raw.k[x], p + tok * (16 * NB) + g * (4 * NB));
-                raw.ks[x] = load_key_scales<NB>(p + 2 * half + tok * NB, g);
-                load_words<NB>(raw.v[x], p + half + quad * (64 * NB) + (lane & 15) * (4 * NB));
-                raw.vs[x] = *reinterpret_cast<const uint32_t *>(p + 2 * half + a.g.page_size * NB + quad * (4 * NB) + v_block<NB>(lane & 15) * 4);
+                const uint32_t in = (t + 16 * x) & mask;
+                const uint8_t *keys = p + in * (16 * NB), *vals = keys + half, *scales = p + 2 * half + in * NB;
+                load_words<NB>(raw.k[x], keys + key_at);
+                raw.ks[x] = load_key_scales<NB>(scales + key_scale_at, g);
+                load_words<NB>(raw.v[x], vals + val_at);
+                raw.vs[x] = *reinterpret_cast<const uint32_t *>(scales + a.g.page_size * NB + val_scale_at);
             }
         };
         auto work = [&](KvRaw<NB> &raw, uint32_t t, const uint32_t *page) {
             const bool there[2] = {page[0] < a.g.pages, page[1] < a.g.pages};
-            if (there[0] && there[1] && t + 32 <= all_see && t + 32 <= t1) {
-                seen_from = min(seen_from, t);
-                r.template step<false>(raw, a.scale_log2, [](int, int, int) { return true; }, [&](int x, int j) { return t + 16 * x + 4 * g + j; });
-            } else {
+            const bool part = !(there[0] && there[1] && t + 32 <= t1);  // some token is none
+            if (there[0]) seen_from = min(seen_from, t);
+            else if (there[1]) seen_from = min(seen_from, t + 16);
+            if (part) {
+                // scales of tokens that are not there (or not in this part): whatever lies in the page must not turn 0 into NaN
 #pragma unroll
                 for (int x = 0; x < 2; ++x) {
-                    if (there[x]) seen_from = min(seen_from, t + 16 * x);
-                    // scales of tokens that are not there (or not in this part): whatever lies in the page must not turn 0 into NaN
                     const uint32_t at = t + 16 * x + 4 * g, live = !there[x] || at >= t1 ? 0 : min(t1 - at, 4u);
                     if (live < 4) raw.vs[x] &= (1u << (8 * live)) - 1;
                 }
-                r.template step<true>(
-                    raw, a.scale_log2,
-                    [&](int row_tile, int x, int j) { const uint32_t at = t + 16 * x + 4 * g + j; return there[x] && at < limit[row_tile] && at < t1; },
-                    [&](int x, int j) { return t + 16 * x + 4 * g + j; });
             }
+            r.step(raw, a.scale_log2, part || t + 32 > all_see,
+                   [&](int row_tile, int x, int j) { const uint32_t at = t + 16 * x + 4 * g + j; return there[x] && at < limit[row_tile] && at < t1; },
+                   [&](int x, int j) { return t + 16 * x + 4 * g + j; });
         };
         KvRaw<NB> cur, nxt;
         uint32_t page[2] = {page_of(t0), page_of(t0 + 16)};
@@ -478,14 +480,15 @@ __global__ __launch_bounds__(256) void k_kv_attend(const KvAttendArgs a) {
     }
 }
 
-// Joins the splits of a row in their order: one wave for a (row, head).
-template <int TERMS>
+// Joins the splits (at most 256) of a row, one block for a (row, head): a thread for each split's maximum and sum, then four columns and
+// every (1024 / W)-th split to a thread.  The order of the sums depends on the sizes alone.  Latency of three dependent reads: the first
+// parts are on their way before the weights are known.
+template <int W, int TERMS>
 __global__ __launch_bounds__(256) void k_kv_join(const KvAttendArgs a) {
-    const uint32_t lane = threadIdx.x & 63, qheads = a.g.heads * a.group;
-    const uint64_t at = (uint64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    const uint32_t head = (uint32_t)(at % qheads), i = (uint32_t)(at / qheads % a.n);
-    const uint64_t j = at / qheads / a.n;
-    if (j >= a.max_new) return;
+    constexpr uint32_t COLS = W / 4, LANES = 256 / COLS, AHEAD = 2;
+    __shared__ float weight[256], red[2][4];
+    __shared__ float4 sum[LANES][COLS];
+    const uint32_t tid = threadIdx.x, qheads = a.g.heads * a.group, head = blockIdx.x % qheads, i = blockIdx.x / qheads % a.n, j = blockIdx.x / qheads / a.n;
     const uint32_t first = min(a.starts[i], a.rows), next = min(a.starts[i + 1], a.rows), count = next > first ? next - first : 0;
     if (j >= count) return;
     const uint32_t length = a.lengths[i];
@@ -495,27 +498,53 @@ __global__ __launch_bounds__(256) void k_kv_join(const KvAttendArgs a) {
     const uint64_t row = (uint64_t)(first + j) * qheads + head;
     const uint32_t live = min((limit + a.split_tokens - 1) / a.split_tokens, a.splits), step = a.g.dim + 4;
     const float *part = a.part + row * a.splits * step;
-    float m = -INFINITY, l = 0;
-    for (uint32_t s = 0; s < live; ++s) m = fmaxf(m, part[s * step + a.g.dim]);
-    const uint32_t d = lane * 4;
-    float o[4] = {};
-    for (uint32_t s = 0; s < live; ++s) {
-        const float ms = part[s * step + a.g.dim];
-        if (ms == -INFINITY) continue;
-        const float by = __builtin_amdgcn_exp2f(ms - m);
-        l += part[s * step + a.g.dim + 1] * by;
-        if (d < a.g.dim) {
-            const float4 x = *reinterpret_cast<const float4 *>(part + s * step + d);
-            o[0] += x.x * by; o[1] += x.y * by; o[2] += x.z * by; o[3] += x.w * by;
-        }
+    const uint32_t lane = tid / COLS, d = tid % COLS * 4;
+    const bool mine = d < a.g.dim;
+    float4 ahead[AHEAD] = {};
+#pragma unroll
+    for (uint32_t u = 0; u < AHEAD; ++u)
+        if (mine && lane + u * LANES < live) ahead[u] = *reinterpret_cast<const float4 *>(part + (lane + u * LANES) * step + d);
+    const float ms = tid < live ? part[tid * step + a.g.dim] : -INFINITY, ls = tid < live ? part[tid * step + a.g.dim + 1] : 0.0f;
+    float m = ms;
+#pragma unroll
+    for (int x = 1; x < 64; x <<= 1) m = fmaxf(m, __shfl_xor(m, x));
+    if ((tid & 63) == 0) red[0][tid >> 6] = m;
+    __syncthreads();
+    m = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
+    const float w = ms == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ms - m);  // (-inf: the split saw nothing and left nothing)
+    weight[tid] = w;
+    float l = ms == -INFINITY ? 0.0f : ls * w;
+#pragma unroll
+    for (int x = 1; x < 64; x <<= 1) l += __shfl_xor(l, x);
+    if ((tid & 63) == 0) red[1][tid >> 6] = l;
+    __syncthreads();
+    float4 o = make_float4(0, 0, 0, 0);
+    auto add = [&](const float4 &x, uint32_t s) {
+        const float by = weight[s];
+        if (by != 0.0f) { o.x += x.x * by; o.y += x.y * by; o.z += x.z * by; o.w += x.w * by; }
+    };
+    if (mine) {
+#pragma unroll
+        for (uint32_t u = 0; u < AHEAD; ++u)
+            if (lane + u * LANES < live) add(ahead[u], lane + u * LANES);
+#pragma unroll 4
+        for (uint32_t s = lane + AHEAD * LANES; s < live; s += LANES) add(*reinterpret_cast<const float4 *>(part + s * step + d), s);
     }
+    sum[lane][tid % COLS] = o;
+    __syncthreads();
+    if (lane != 0) return;
+#pragma unroll
+    for (uint32_t u = 1; u < LANES; ++u) {
+        const float4 x = sum[u][tid % COLS];
+        o.x += x.x; o.y += x.y; o.z += x.z; o.w += x.w;
+    }
+    l = (red[1][0] + red[1][1]) + (red[1][2] + red[1][3]);
     const bool some = m != -INFINITY;
     const float by = some ? 1.0f / l : 0.0f;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) o[e] *= by;
+    const float y[4] = {o.x * by, o.y * by, o.z * by, o.w * by};
     constexpr uint32_t kSize = TERMS == 1 ? 2 : 4;
-    if (d < a.g.dim) store_columns<2, TERMS>(static_cast<uint8_t *>(a.out) + row * a.g.dim * kSize, d, a.g.dim, o);
-    if (lane == 0 && a.lse) a.lse[row] = some ? lse_of(m, l) : -INFINITY;
+    if (mine) store_columns<2, TERMS>(static_cast<uint8_t *>(a.out) + row * a.g.dim * kSize, d, a.g.dim, y);
+    if (tid == 0 && a.lse) a.lse[row] = some ? lse_of(m, l) : -INFINITY;
 }
 
 // ---- attention over selected rows ---------------------------------------------------------------------------------------
@@ -587,7 +616,7 @@ __global__ __launch_bounds__(256) void k_kv_attend_selected(const KvAttendArgs a
                     any |= seen[4 * x + j];
                 }
             }
-            r.template step<true>(raw, a.scale_log2, [&](int, int x, int j) { return seen[4 * x + j]; }, [](int, int) { return 0u; });
+            r.step(raw, a.scale_log2, true, [&](int, int x, int j) { return seen[4 * x + j]; }, [](int, int) { return 0u; });
         }
     }
     r.close();
@@ -624,7 +653,7 @@ static KvCut kv_cut(const KvGeom &g, uint32_t type, uint32_t group, uint32_t n, 
     const uint64_t rows = (uint64_t)max_new * group;
     const uint32_t w = kv_width(g.dim);
     c.wide = rows > 64;
-    c.nt = !c.wide ? 1 : type == ZVDB_KV_F32 ? (w == 256 ? 1 : 2) : w == 256 ? 2 : 4;
+    c.nt = c.wide ? wide_tiles(w / 32, type == ZVDB_KV_F32 ? 3 : 1) : 1;
     const uint32_t block_rows = c.wide ? 64 * c.nt : 16;
     c.tiles = (uint32_t)((rows + block_rows - 1) / block_rows);
     const uint64_t base = (uint64_t)g.heads * n * c.tiles;
@@ -643,12 +672,18 @@ template <int NB>
 static void launch_attend(const KvAttendArgs &a, const KvCut &c, uint32_t type, hipStream_t s) {
     const dim3 grid((uint32_t)c.blocks), block(256);
     if (type == ZVDB_KV_F32) {
-        if (c.wide) hipLaunchKernelGGL((k_kv_attend<NB, NB == 8 ? 1 : 2, 3, true>), grid, block, 0, s, a);
+        if (c.wide) hipLaunchKernelGGL((k_kv_attend<NB, wide_tiles(NB, 3), 3, true>), grid, block, 0, s, a);
         else hipLaunchKernelGGL((k_kv_attend<NB, 1, 3, false>), grid, block, 0, s, a);
     } else {
-        if (c.wide) hipLaunchKernelGGL((k_kv_attend<NB, NB == 8 ? 2 : 4, 1, true>), grid, block, 0, s, a);
+        if (c.wide) hipLaunchKernelGGL((k_kv_attend<NB, wide_tiles(NB, 1), 1, true>), grid, block, 0, s, a);
         else hipLaunchKernelGGL((k_kv_attend<NB, 1, 1, false>), grid, block, 0, s, a);
     }
+}
+
+template <int W>
+static void launch_join(const KvAttendArgs &a, uint32_t blocks, uint32_t type, hipStream_t s) {
+    if (type == ZVDB_KV_F32) hipLaunchKernelGGL((k_kv_join<W, 3>), dim3(blocks), dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((k_kv_join<W, 1>), dim3(blocks), dim3(256), 0, s, a);
 }
 
 template <int NB>
@@ -749,10 +784,11 @@ int zvdb_hip_kv_attend_dev(const zvdb_hip_kv_layout *layout, const void *d_cache
     else launch_attend<8>(a, c, type, s);
     ZV_HIP(hipGetLastError());
     if (c.splits > 1) {
-        const uint64_t blocks = ((uint64_t)q_heads * n * max_new + 3) / 4;
+        const uint64_t blocks = (uint64_t)q_heads * n * max_new;
         KV_ARG(blocks < 0x7FFFFFFFull, "kv_attend: the call is too large (%llu rows)", (unsigned long long)blocks);
-        if (type == ZVDB_KV_F32) hipLaunchKernelGGL((k_kv_join<3>), dim3((uint32_t)blocks), dim3(256), 0, s, a);
-        else hipLaunchKernelGGL((k_kv_join<1>), dim3((uint32_t)blocks), dim3(256), 0, s, a);
+        if (w == 64) launch_join<64>(a, (uint32_t)blocks, type, s);
+        else if (w == 128) launch_join<128>(a, (uint32_t)blocks, type, s);
+        else launch_join<256>(a, (uint32_t)blocks, type, s);
         ZV_HIP(hipGetLastError());
     }
     return ZVDB_OK;
