@@ -335,7 +335,9 @@ __device__ inline void join_waves(KvRows<NB, 1, TERMS> &r) {
 // A block takes row tile(s) x one key/value head x one split of the tokens of a request.  WIDE = false (few rows: decode): its four
 // waves share 16 rows and divide the split's tokens, joined in LDS.  WIDE = true (prompts): each wave has NT tiles of its own and
 // walks the same tokens.  Blocks are numbered head first, so that (with 8 heads) an XCD's L2 keeps the pages of its own heads,
-// and row tiles last to first, so that the causal ones with most tokens start first.
+// and row tiles last to first, so that the causal ones with most tokens start first.  The requests turn by one from one tile or split to
+// the next: blocks are dealt to the shader engines in order, and without it one of them gets all of a long request (4 prompts: 465 us, a
+// third of the wave slots empty).
 template <int NB, int NT, int TERMS, bool WIDE>
 __global__ __launch_bounds__(256, NB == 8 && TERMS == 3 ? 1 : WIDE || NB == 8 || TERMS == 3 ? 2 : 4) void k_kv_attend(const KvAttendArgs a) {
     static_assert(WIDE || NT == 1, "waves that share rows hold one tile");
@@ -343,9 +345,7 @@ __global__ __launch_bounds__(256, NB == 8 && TERMS == 3 ? 1 : WIDE || NB == 8 ||
     uint32_t b = blockIdx.x;
     const uint32_t head = b % a.g.heads;
     b /= a.g.heads;
-    const uint32_t split = b % a.splits;
-    b /= a.splits;
-    const uint32_t i = b % a.n, tile = a.tiles - 1 - b / a.n;
+    const uint32_t turn = b / a.n, i = (b + turn) % a.n, split = turn % a.splits, tile = a.tiles - 1 - turn / a.splits;
 
     // the request: rows [first, first + count) of q, `length` tokens, of which those up to `end` are reachable
     const uint32_t first = min(a.starts[i], a.rows), next = min(a.starts[i + 1], a.rows), count = next > first ? next - first : 0;
