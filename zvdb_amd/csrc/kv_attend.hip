@@ -41,8 +41,6 @@ struct KvAttendArgs {
     bool causal;
 };
 
-// Row tiles of a wave when a prompt gives every wave its own: as many as its registers hold beside two chunks of raw rows, with two waves on a SIMD
-constexpr int wide_tiles(int nb, int terms) { return terms == 1 && nb <= 4 ? 3 : 1; }
 constexpr float kSlack = 8.0f;
 constexpr float kNone = -FLT_MAX;  // maximum of a row that has seen nothing: exp2(-inf - kNone) = 0, never NaN
 constexpr float kLn2 = 0.693147180559945309f;
@@ -100,6 +98,51 @@ __device__ inline void split_bf16(const float *x, bf16x8 *t) {  // x[8] = t[0] +
     }
 }
 
+// 8 codes of a key row
+__device__ inline bf16x8 widen_key(uint32_t w, float scale) {
+    const bf16x2 c0 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 0), c1 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 1),
+                 c2 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 2), c3 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 3);
+    return bf16x8{c0[0], c0[1], c1[0], c1[1], c2[0], c2[1], c3[0], c3[1]};
+}
+
+// Byte b (columns 2 b and 2 b + 1) of one piece of four tokens' values v: the four tokens of each column
+template <int NB>
+__device__ inline void widen_values(const uint32_t *v, const float *scale, int b, uint2 &lo, uint2 &hi) {
+    uint32_t w[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const uint32_t src = v[(j * NB + b) / 4];
+        bf16x2 c;
+        switch ((j * NB + b) % 4) {
+            case 0: c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(src, scale[j], 0); break;
+            case 1: c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(src, scale[j], 1); break;
+            case 2: c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(src, scale[j], 2); break;
+            default: c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(src, scale[j], 3); break;
+        }
+        w[j] = __builtin_bit_cast(uint32_t, c);
+    }
+    lo.x = __builtin_amdgcn_perm(w[1], w[0], 0x05040100u); hi.x = __builtin_amdgcn_perm(w[1], w[0], 0x07060302u);
+    lo.y = __builtin_amdgcn_perm(w[3], w[2], 0x05040100u); hi.y = __builtin_amdgcn_perm(w[3], w[2], 0x07060302u);
+}
+
+// Scales of 4 N tokens' value blocks.  A NaN block counts as 0, so that rows that do not see its token stay whole; the smallest index of
+// such a token is returned (~0: none).  All 64 lanes call this.
+template <int N, class Token>
+__device__ inline uint32_t value_scales(const uint32_t *words, float *vs, Token token) {
+    uint32_t nan = ~0u;
+#pragma unroll
+    for (int j = 0; j < 4 * N; ++j) vs[j] = pow2_of(words[j / 4], j % 4);
+    float top = vs[0];
+#pragma unroll
+    for (int j = 1; j < 4 * N; ++j) top = fmaxf(top, vs[j]);
+    if (__any(top == INFINITY)) {
+#pragma unroll
+        for (int j = 0; j < 4 * N; ++j)
+            if (vs[j] == INFINITY) { vs[j] = 0.0f; nan = min(nan, token(j / 4, j % 4)); }
+    }
+    return nan;
+}
+
 // The state of NT tiles of 16 rows in a wave
 template <int NB, int NT, int TERMS>
 struct KvRows {
@@ -144,57 +187,56 @@ struct KvRows {
         }
     }
 
-    // `seen(t, i, j)`: whether this lane's row of row tile t sees token 4 g + j of token tile i; asked only where `mask` (uniform).
-    // `token(i, j)`: the index that nan_at counts of that token.
-    template <class Seen, class Token>
-    __device__ void step(const KvRaw<NB> &raw, float scale_log2, bool mask, Seen seen, Token token) {
-        // V's scales; a NaN block counts as 0 here and is entered in nan_at, so that rows that do not see its token stay whole
-        float vs[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) vs[j] = pow2_of(raw.vs[j / 4], j % 4);
-        float top = vs[0];
-#pragma unroll
-        for (int j = 1; j < 8; ++j) top = fmaxf(top, vs[j]);
-        if (__any(top == INFINITY)) {
-#pragma unroll
-            for (int j = 0; j < 8; ++j)
-                if (vs[j] == INFINITY) { vs[j] = 0.0f; nan_at = min(nan_at, token(j / 4, j % 4)); }
-        }
-        f32x4 s[NT][2];
+    // S^T of 32 tokens: key(i, b) is the A operand of token tile i and step b
+    template <class Key>
+    __device__ void scores(f32x4 (*s)[2], Key key) const {
 #pragma unroll
         for (int t = 0; t < NT; ++t) s[t][0] = s[t][1] = f32x4{0, 0, 0, 0};
 #pragma unroll
         for (int i = 0; i < 2; ++i)
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
-                const float ks = pow2_of(raw.ks[i], NB == 8 ? b / 4 : 0);
-                const bf16x2 c0 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(raw.k[i][b], ks, 0), c1 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(raw.k[i][b], ks, 1),
-                             c2 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(raw.k[i][b], ks, 2), c3 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(raw.k[i][b], ks, 3);
-                const bf16x8 a = {c0[0], c0[1], c1[0], c1[1], c2[0], c2[1], c3[0], c3[1]};
+                const bf16x8 a = key(i, b);
 #pragma unroll
                 for (int t = 0; t < NT; ++t)
 #pragma unroll
                     for (int n = TERMS - 1; n >= 0; --n) s[t][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, q[t][n][b], s[t][i], 0, 0, 0);
             }
-        bf16x8 p[NT][TERMS];
+    }
+
+    // Scores to weights.  `seen(t, i, j)`: whether this lane's row of row tile t sees token 4 g + j of token tile i; asked only where
+    // `mask` (uniform).
+    template <class Seen>
+    __device__ void weights(f32x4 (*s)[2], bf16x8 (*p)[TERMS], float scale_log2, bool mask, Seen seen) {
+        if (mask) {
 #pragma unroll
-        for (int t = 0; t < NT; ++t) {
-            if (mask) {
+            for (int t = 0; t < NT; ++t)
 #pragma unroll
                 for (int j = 0; j < 8; ++j)
                     if (!seen(t, j / 4, j % 4)) s[t][j / 4][j % 4] = -INFINITY;
-            }
-            float mx = s[t][0][0];
+        }
+        float mx[NT];
+        bool over = false;
 #pragma unroll
-            for (int j = 1; j < 8; ++j) mx = fmaxf(mx, s[t][j / 4][j % 4]);
-            mx *= scale_log2;
-            if (__any(mx > m[t] + kSlack)) {
-                const float to = fmaxf(m[t], max_over_row(mx)), by = __builtin_amdgcn_exp2f(m[t] - to);
+        for (int t = 0; t < NT; ++t) {
+            mx[t] = s[t][0][0];
+#pragma unroll
+            for (int j = 1; j < 8; ++j) mx[t] = fmaxf(mx[t], s[t][j / 4][j % 4]);
+            mx[t] *= scale_log2;
+            over |= mx[t] > m[t] + kSlack;
+        }
+        if (__any(over)) {
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+                const float to = fmaxf(m[t], max_over_row(mx[t])), by = __builtin_amdgcn_exp2f(m[t] - to);
                 m[t] = to;
                 l[t] *= by;
 #pragma unroll
                 for (int i = 0; i < 2 * NB; ++i) o[t][i] *= by;
             }
+        }
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
             float x[8];
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
@@ -203,37 +245,41 @@ struct KvRows {
             }
             split_bf16<TERMS>(x, p[t]);
         }
-        // byte b of a piece holds columns 2 b and 2 b + 1 of one token: widen 8 tokens, then sort the pairs by column
+    }
+
+    // O^T += V^T P^T: value(b, a) gives the A operands of columns 2 b and 2 b + 1 of the pieces
+    template <class Value>
+    __device__ void products(const bf16x8 (*p)[TERMS], Value value) {
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
-            uint32_t w[8];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const int byte = (j % 4) * NB + b;
-                const uint32_t src = raw.v[j / 4][byte / 4];
-                bf16x2 c;
-                switch (byte % 4) {
-                    case 0: c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(src, vs[j], 0); break;
-                    case 1: c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(src, vs[j], 1); break;
-                    case 2: c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(src, vs[j], 2); break;
-                    default: c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(src, vs[j], 3); break;
-                }
-                w[j] = __builtin_bit_cast(uint32_t, c);
-            }
-            uint4 lo, hi;
-            lo.x = __builtin_amdgcn_perm(w[1], w[0], 0x05040100u); hi.x = __builtin_amdgcn_perm(w[1], w[0], 0x07060302u);
-            lo.y = __builtin_amdgcn_perm(w[3], w[2], 0x05040100u); hi.y = __builtin_amdgcn_perm(w[3], w[2], 0x07060302u);
-            lo.z = __builtin_amdgcn_perm(w[5], w[4], 0x05040100u); hi.z = __builtin_amdgcn_perm(w[5], w[4], 0x07060302u);
-            lo.w = __builtin_amdgcn_perm(w[7], w[6], 0x05040100u); hi.w = __builtin_amdgcn_perm(w[7], w[6], 0x07060302u);
-            const bf16x8 a0 = __builtin_bit_cast(bf16x8, lo), a1 = __builtin_bit_cast(bf16x8, hi);
+            bf16x8 a[2];
+            value(b, a);
 #pragma unroll
             for (int t = 0; t < NT; ++t)
 #pragma unroll
                 for (int n = TERMS - 1; n >= 0; --n) {
-                    o[t][2 * b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a0, p[t][n], o[t][2 * b], 0, 0, 0);
-                    o[t][2 * b + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a1, p[t][n], o[t][2 * b + 1], 0, 0, 0);
+                    o[t][2 * b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[0], p[t][n], o[t][2 * b], 0, 0, 0);
+                    o[t][2 * b + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[1], p[t][n], o[t][2 * b + 1], 0, 0, 0);
                 }
         }
+    }
+
+    // 32 tokens that this wave widens for itself; `token(i, j)`: the index that nan_at counts of token 4 g + j of token tile i
+    template <class Seen, class Token>
+    __device__ void step(const KvRaw<NB> &raw, float scale_log2, bool mask, Seen seen, Token token) {
+        float vs[8];
+        nan_at = min(nan_at, value_scales<2>(raw.vs, vs, token));
+        f32x4 s[NT][2];
+        scores(s, [&](int i, int b) { return widen_key(raw.k[i][b], pow2_of(raw.ks[i], NB == 8 ? b / 4 : 0)); });
+        bf16x8 p[NT][TERMS];
+        weights(s, p, scale_log2, mask, seen);
+        products(p, [&](int b, bf16x8 *a) {
+            uint2 lo[2], hi[2];
+            widen_values<NB>(raw.v[0], vs, b, lo[0], hi[0]);
+            widen_values<NB>(raw.v[1], vs + 4, b, lo[1], hi[1]);
+            a[0] = __builtin_bit_cast(bf16x8, make_uint4(lo[0].x, lo[0].y, lo[1].x, lo[1].y));
+            a[1] = __builtin_bit_cast(bf16x8, make_uint4(hi[0].x, hi[0].y, hi[1].x, hi[1].y));
+        });
     }
 
     __device__ void close() {  // sums of a row's four lanes
@@ -289,6 +335,13 @@ __device__ inline void store_columns(void *row, uint32_t d, uint32_t dim, const 
     }
 }
 
+// The scale bytes of the four tokens from `at` on that are there (before t1, in a page): whatever lies in the place of the others must not
+// turn 0 into NaN
+__device__ inline uint32_t live_scales(bool there, uint32_t at, uint32_t t1) {
+    const uint32_t live = !there || at >= t1 ? 0 : min(t1 - at, 4u);
+    return live == 4 ? ~0u : (1u << (8 * live)) - 1;
+}
+
 __device__ inline float lse_of(float m, float l) { return (m + __log2f(l)) * kLn2; }
 
 // Joins the four waves of a block, each with its own tokens, in wave 0 (all 256 threads call this).  Sums in a fixed order.
@@ -332,152 +385,292 @@ __device__ inline void join_waves(KvRows<NB, 1, TERMS> &r) {
 
 // ---- attention over whole requests --------------------------------------------------------------------------------------
 
-// A block takes row tile(s) x one key/value head x one split of the tokens of a request.  WIDE = false (few rows: decode): its four
-// waves share 16 rows and divide the split's tokens, joined in LDS.  WIDE = true (prompts): each wave has NT tiles of its own and
-// walks the same tokens.  Blocks are numbered head first, so that (with 8 heads) an XCD's L2 keeps the pages of its own heads,
-// and row tiles last to first, so that the causal ones with most tokens start first.  The requests turn by one from one tile or split to
-// the next: blocks are dealt to the shader engines in order, and without it one of them gets all of a long request (4 prompts: 465 us, a
-// third of the wave slots empty).
-template <int NB, int NT, int TERMS, bool WIDE>
-__global__ __launch_bounds__(256, NB == 8 && TERMS == 3 ? 1 : WIDE || NB == 8 || TERMS == 3 ? 2 : 4) void k_kv_attend(const KvAttendArgs a) {
-    static_assert(WIDE || NT == 1, "waves that share rows hold one tile");
-    const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4;
-    uint32_t b = blockIdx.x;
-    const uint32_t head = b % a.g.heads;
-    b /= a.g.heads;
-    const uint32_t turn = b / a.n, i = (b + turn) % a.n, split = turn % a.splits, tile = a.tiles - 1 - turn / a.splits;
+// What a block of k_kv_attend / k_kv_attend_wide works on: row tile x one key/value head x one split of the tokens of a request.  Blocks are
+// numbered head first, so that (with 8 heads) an XCD's L2 keeps the pages of its own heads, and row tiles last to first, so that the
+// causal ones with most tokens start first.  The requests turn by one from one tile or split to the next: blocks are dealt to the shader
+// engines in order, and without it one of them gets all of a long request (4 prompts: 465 -> 331 us).
+struct KvBlock {
+    uint32_t head, i, split, first, count, length, reach, rows, row0, end;
 
-    // the request: rows [first, first + count) of q, `length` tokens, of which those up to `end` are reachable
-    const uint32_t first = min(a.starts[i], a.rows), next = min(a.starts[i + 1], a.rows), count = next > first ? next - first : 0;
-    const uint32_t length = a.lengths[i];
-    const uint32_t reach = (uint32_t)min((uint64_t)min(length, a.max_length), (uint64_t)a.table_stride << a.g.page_shift);
-    const uint32_t rows = min(count, a.max_new) * a.group;
-    constexpr uint32_t kWaveRows = 16 * NT;
-    const uint32_t block_row = tile * (WIDE ? 4 * kWaveRows : 16);
-    if (block_row >= rows) return;
-    const uint32_t wave_row = block_row + (WIDE ? wave * kWaveRows : 0);
-    // a row's limit: the tokens it sees are [0, limit)
-    auto limit_of = [&](uint32_t row) {
+    __device__ KvBlock(const KvAttendArgs &a, uint32_t block_rows) {
+        const uint32_t b = blockIdx.x / a.g.heads, turn = b / a.n;
+        head = blockIdx.x % a.g.heads;
+        i = (b + turn) % a.n;
+        split = turn % a.splits;
+        row0 = (a.tiles - 1 - turn / a.splits) * block_rows;
+        // rows [first, first + count) of q, `length` tokens, of which those below `reach` can be read
+        first = min(a.starts[i], a.rows);
+        const uint32_t next = min(a.starts[i + 1], a.rows);
+        count = next > first ? next - first : 0;
+        length = a.lengths[i];
+        reach = (uint32_t)min((uint64_t)min(length, a.max_length), (uint64_t)a.table_stride << a.g.page_shift);
+        rows = min(count, a.max_new) * a.group;
+        end = row0 < rows ? limit(a, min(row0 + block_rows, rows) - 1) : 0;  // no row of the block sees more
+    }
+    __device__ uint32_t limit(const KvAttendArgs &a, uint32_t row) const {  // the tokens a row sees are [0, limit)
         if (!a.causal) return reach;
         const int64_t x = (int64_t)length - count + row / a.group + 1;
         return (uint32_t)min(max(x, (int64_t)0), (int64_t)reach);
-    };
-    const uint32_t block_end = limit_of(min(block_row + (WIDE ? 4 * kWaveRows : 16), rows) - 1);
-    uint32_t t0 = split * a.split_tokens;
-    if (a.splits > 1 && t0 >= block_end) return;  // (no row of the block sees a token of this split: k_kv_join knows)
-    uint32_t t1 = a.splits > 1 ? min(t0 + a.split_tokens, block_end) : block_end;
-    if (WIDE) {
-        if (wave_row >= rows) return;
-        t1 = min(t1, limit_of(min(wave_row + kWaveRows, rows) - 1));
-    } else {  // this wave's quarter, in whole chunks
-        const uint32_t part = ((t1 - t0 + 127) >> 7) << 5;
-        t0 = min(t0 + wave * part, t1);
-        t1 = min(t0 + part, t1);
     }
-
-    KvRows<NB, NT, TERMS> r;
-    r.clear();
-    uint32_t limit[NT];
-    const uint32_t qheads = a.g.heads * a.group;
-    constexpr uint32_t kSize = TERMS == 1 ? 2 : 4;
-#pragma unroll
-    for (int t = 0; t < NT; ++t) {
-        const uint32_t row = wave_row + t * 16 + (lane & 15);
-        limit[t] = row < rows ? limit_of(row) : 0;
-        const uint8_t *p = static_cast<const uint8_t *>(a.q) + ((uint64_t)(first + row / a.group) * a.q_stride + (uint64_t)(head * a.group + row % a.group) * a.g.dim) * kSize;
-        r.load_q(t, row < rows ? p : nullptr, a.g.dim);
+    __device__ const void *query(const KvAttendArgs &a, uint32_t row, uint32_t size) const {
+        if (row >= rows) return nullptr;
+        return static_cast<const uint8_t *>(a.q) + ((uint64_t)(first + row / a.group) * a.q_stride + (uint64_t)(head * a.group + row % a.group) * a.g.dim) * size;
     }
-    const uint32_t all_see = __builtin_amdgcn_readfirstlane(limit_of(min(wave_row, rows - 1)));  // rows behind the last one do not count: they are not stored
-    uint32_t seen_from = ~0u;  // first token of the first page that is there
+    // place of a row in out (times head_dim) and lse
+    __device__ uint64_t place(const KvAttendArgs &a, uint32_t row) const { return (uint64_t)(first + row / a.group) * (a.g.heads * a.group) + head * a.group + row % a.group; }
+};
 
-    if (t0 < t1) {
-        const uint32_t *table = a.tables + (uint64_t)i * a.table_stride;
-        const uint32_t last_page = (t1 - 1) >> a.g.page_shift, half = a.g.page_size * 16 * NB, mask = a.g.page_size - 1;
-        const uint8_t *heads = a.cache + (uint64_t)head * a.g.head_bytes;
-        const uint32_t chunks = (t1 - t0 + 31) >> 5;
-        auto page_of = [&](uint32_t t) { return table[min(t >> a.g.page_shift, last_page)]; };
-        // what a lane adds to a tile's place: the rest of an address is uniform
-        const uint32_t key_at = (lane & 15) * (16 * NB) + g * (4 * NB), key_scale_at = (lane & 15) * NB, val_at = g * (64 * NB) + (lane & 15) * (4 * NB),
-                       val_scale_at = g * (4 * NB) + v_block<NB>(lane & 15) * 4;
-        auto load = [&](KvRaw<NB> &raw, uint32_t t, const uint32_t *page) {
-#pragma unroll
-            for (int x = 0; x < 2; ++x) {
-                const uint8_t *p = heads + (uint64_t)(page[x] < a.g.pages ? page[x] : 0) * a.g.page_bytes;
-                const uint32_t in = (t + 16 * x) & mask;
-                const uint8_t *keys = p + in * (16 * NB), *vals = keys + half, *scales = p + 2 * half + in * NB;
-                load_words<NB>(raw.k[x], keys + key_at);
-                raw.ks[x] = load_key_scales<NB>(scales + key_scale_at, g);
-                load_words<NB>(raw.v[x], vals + val_at);
-                raw.vs[x] = *reinterpret_cast<const uint32_t *>(scales + a.g.page_size * NB + val_scale_at);
-            }
-        };
-        auto work = [&](KvRaw<NB> &raw, uint32_t t, const uint32_t *page) {
-            const bool there[2] = {page[0] < a.g.pages, page[1] < a.g.pages};
-            const bool part = !(there[0] && there[1] && t + 32 <= t1);  // some token is none
-            if (there[0]) seen_from = min(seen_from, t);
-            else if (there[1]) seen_from = min(seen_from, t + 16);
-            if (part) {
-                // scales of tokens that are not there (or not in this part): whatever lies in the page must not turn 0 into NaN
-#pragma unroll
-                for (int x = 0; x < 2; ++x) {
-                    const uint32_t at = t + 16 * x + 4 * g, live = !there[x] || at >= t1 ? 0 : min(t1 - at, 4u);
-                    if (live < 4) raw.vs[x] &= (1u << (8 * live)) - 1;
-                }
-            }
-            r.step(raw, a.scale_log2, part || t + 32 > all_see,
-                   [&](int row_tile, int x, int j) { const uint32_t at = t + 16 * x + 4 * g + j; return there[x] && at < limit[row_tile] && at < t1; },
-                   [&](int x, int j) { return t + 16 * x + 4 * g + j; });
-        };
-        KvRaw<NB> cur, nxt;
-        uint32_t page[2] = {page_of(t0), page_of(t0 + 16)};
-        load(cur, t0, page);
-        for (uint32_t c = 0; c < chunks; ++c) {
-            const uint32_t t = t0 + c * 32, tn = min(t + 32, t0 + (chunks - 1) * 32);
-            const uint32_t pn[2] = {page_of(tn), page_of(tn + 16)};
-            load(nxt, tn, pn);
-            work(cur, t, page);
-            cur = nxt;
-            page[0] = pn[0];
-            page[1] = pn[1];
+// The pages of the tiles (16 tokens) from `t0` on, gone through in order: 64 of them lie in a register, one to a lane, and the next 64 are
+// on their way, so that no load of a page waits for its number.  (All 64 lanes call these; tiles behind the last page get the last.)
+struct KvPages {
+    const uint32_t *table;
+    uint32_t t0, last, shift, pages, base, ids, next;
+    uint64_t are;
+
+    __device__ KvPages(const KvAttendArgs &a, uint32_t request, uint32_t from, uint32_t to)
+        : table(a.tables + (uint64_t)request * a.table_stride), t0(from), last((to - 1) >> a.g.page_shift), shift(a.g.page_shift), pages(a.g.pages), base(0) {
+        next = read(0);
+        take();
+    }
+    __device__ uint32_t read(uint32_t tile) const { return table[min((t0 + 16 * (tile + (threadIdx.x & 63))) >> shift, last)]; }
+    __device__ void take() {
+        are = __ballot(next < pages);
+        ids = next < pages ? next : 0;
+        next = read(base + 64);
+    }
+    __device__ void reach(uint32_t tile) {  // before anything is asked about the tiles from `tile` (uniform) to the next multiple of 64
+        if (tile >= base + 64) {
+            base += 64;
+            take();
         }
     }
-    r.close();
-    if constexpr (!WIDE) {
-        __shared__ uint32_t from[4];
-        if (lane == 0) from[wave] = seen_from;
-        join_waves<NB, TERMS>(r);
-        if (wave != 0) return;
-        seen_from = min(min(from[0], from[1]), min(from[2], from[3]));
-    }
+    __device__ uint32_t page(uint32_t tile) const { return __builtin_amdgcn_readlane(ids, tile - base); }  // 0 where there is none
+    __device__ uint32_t there(uint32_t tile) const { return (uint32_t)(are >> (tile - base)); }            // bit 0: the tile has a page; bit 1: the next; ...
+};
+
+// Writes a wave's rows: the result, or (several splits) the part that k_kv_join joins
+template <int NB, int NT, int TERMS>
+__device__ inline void store_rows(const KvAttendArgs &a, const KvBlock &blk, const KvRows<NB, NT, TERMS> &r, const uint32_t *limit, uint32_t wave_row, uint32_t seen_from) {
+    constexpr uint32_t kSize = TERMS == 1 ? 2 : 4;
+    const uint32_t lane = threadIdx.x & 63, g = lane >> 4;
     uint32_t nan_first[4];
     nan_blocks<NB>(r.nan_at, nan_first);
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
         const uint32_t row = wave_row + t * 16 + (lane & 15);
-        if (row >= rows) continue;
-        const uint64_t out_row = (uint64_t)(first + row / a.group) * qheads + head * a.group + row % a.group;
-        const bool some = seen_from < limit[t];
-        const bool whole = a.splits == 1;
+        if (row >= blk.rows) continue;
+        const uint64_t at = blk.place(a, row);
+        const bool some = seen_from < limit[t], whole = a.splits == 1;
         const float by = whole ? (some ? 1.0f / r.l[t] : 0.0f) : 1.0f;
+        float *part = a.part + (at * a.splits + blk.split) * (a.g.dim + 4);
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
             float y[2 * NB];
 #pragma unroll
             for (int e = 0; e < 2 * NB; ++e) y[e] = nan_first[x] < limit[t] ? __uint_as_float(0x7FC00000u) : r.o[t][e][x] * by;
             const uint32_t d = (4 * g + x) * 2 * NB;
-            if (whole) store_columns<NB, TERMS>(static_cast<uint8_t *>(a.out) + out_row * a.g.dim * kSize, d, a.g.dim, y);
-            else store_columns<NB, 3>(a.part + (out_row * a.splits + split) * (a.g.dim + 4), d, a.g.dim, y);
+            if (whole) store_columns<NB, TERMS>(static_cast<uint8_t *>(a.out) + at * a.g.dim * kSize, d, a.g.dim, y);
+            else store_columns<NB, 3>(part, d, a.g.dim, y);
         }
         if (g == 0) {
             if (!whole) {
-                float *p = a.part + (out_row * a.splits + split) * (a.g.dim + 4) + a.g.dim;
-                p[0] = some ? r.m[t] : -INFINITY;  // -inf: this split saw nothing
-                p[1] = r.l[t];
+                part[a.g.dim] = some ? r.m[t] : -INFINITY;  // -inf: this split saw nothing
+                part[a.g.dim + 1] = r.l[t];
             } else if (a.lse) {
-                a.lse[out_row] = some ? lse_of(r.m[t], r.l[t]) : -INFINITY;
+                a.lse[at] = some ? lse_of(r.m[t], r.l[t]) : -INFINITY;
             }
         }
     }
+}
+
+// Few rows (decode): 16 of them to a block, whose four waves divide the split's tokens and are joined in LDS.  Each wave widens what it
+// loads, one chunk of 32 tokens ahead.
+template <int NB, int TERMS>
+__global__ __launch_bounds__(256, NB == 8 && TERMS == 3 ? 1 : NB == 8 || TERMS == 3 ? 2 : NB == 4 ? 3 : 4) void k_kv_attend(const KvAttendArgs a) {
+    const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4;
+    const KvBlock blk(a, 16);
+    if (blk.row0 >= blk.rows) return;
+    uint32_t t0 = blk.split * a.split_tokens;
+    if (a.splits > 1 && t0 >= blk.end) return;  // (no row of the block sees a token of this split: k_kv_join knows)
+    uint32_t t1 = a.splits > 1 ? min(t0 + a.split_tokens, blk.end) : blk.end;
+    const uint32_t quarter = ((t1 - t0 + 127) >> 7) << 5;  // this wave's, in whole chunks
+    t0 = min(t0 + wave * quarter, t1);
+    t1 = min(t0 + quarter, t1);
+
+    KvRows<NB, 1, TERMS> r;
+    r.clear();
+    const uint32_t row = blk.row0 + (lane & 15), limit = row < blk.rows ? blk.limit(a, row) : 0;
+    r.load_q(0, blk.query(a, row, TERMS == 1 ? 2 : 4), a.g.dim);
+    const uint32_t all_see = __builtin_amdgcn_readfirstlane(blk.limit(a, blk.row0));  // rows behind the last one do not count: they are not stored
+    uint32_t seen_from = ~0u;  // first token of the first page that is there
+
+    if (t0 < t1) {
+        const uint32_t half = a.g.page_size * 16 * NB, mask = a.g.page_size - 1;
+        const uint8_t *heads = a.cache + (uint64_t)blk.head * a.g.head_bytes;
+        const uint32_t chunks = (t1 - t0 + 31) >> 5;
+        KvPages pages(a, blk.i, t0, t1);
+        // what a lane adds to a tile's place: the rest of an address is uniform
+        const uint32_t key_at = (lane & 15) * (16 * NB) + g * (4 * NB), key_scale_at = (lane & 15) * NB, val_at = g * (64 * NB) + (lane & 15) * (4 * NB),
+                       val_scale_at = g * (4 * NB) + v_block<NB>(lane & 15) * 4;
+        auto load = [&](KvRaw<NB> &raw, uint32_t c) -> uint32_t {
+            pages.reach(2 * c);
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+                const uint8_t *p = heads + pages.page(2 * c + x) * a.g.page_bytes;
+                const uint32_t in = (t0 + 32 * c + 16 * x) & mask;
+                const uint8_t *keys = p + in * (16 * NB), *vals = keys + half, *scales = p + 2 * half + in * NB;
+                load_words<NB>(raw.k[x], keys + key_at);
+                raw.ks[x] = load_key_scales<NB>(scales + key_scale_at, g);
+                load_words<NB>(raw.v[x], vals + val_at);
+                raw.vs[x] = *reinterpret_cast<const uint32_t *>(scales + a.g.page_size * NB + val_scale_at);
+            }
+            return pages.there(2 * c) & 3;
+        };
+        auto work = [&](KvRaw<NB> &raw, uint32_t t, uint32_t there) {
+            const bool part = there != 3 || t + 32 > t1;  // some token is none
+            if (there) seen_from = min(seen_from, t + (there & 1 ? 0 : 16));
+            if (part) {
+#pragma unroll
+                for (int x = 0; x < 2; ++x) raw.vs[x] &= live_scales(there >> x & 1, t + 16 * x + 4 * g, t1);
+            }
+            r.step(raw, a.scale_log2, part || t + 32 > all_see,
+                   [&](int, int x, int j) { const uint32_t at = t + 16 * x + 4 * g + j; return (there >> x & 1) && at < limit && at < t1; },
+                   [&](int x, int j) { return t + 16 * x + 4 * g + j; });
+        };
+        KvRaw<NB> cur, nxt;
+        uint32_t there = load(cur, 0);
+        for (uint32_t c = 0; c < chunks; ++c) {
+            const uint32_t there_next = load(nxt, min(c + 1, chunks - 1));
+            work(cur, t0 + c * 32, there);
+            cur = nxt;
+            there = there_next;
+        }
+    }
+    r.close();
+    __shared__ uint32_t from[4];
+    if (lane == 0) from[wave] = seen_from;
+    join_waves<NB, TERMS>(r);
+    if (wave != 0) return;
+    store_rows(a, blk, r, &limit, blk.row0, min(min(from[0], from[1]), min(from[2], from[3])));
+}
+
+// Row tiles of a wave of k_kv_attend_wide: what 256 registers hold
+constexpr int wide_tiles(int nb, int terms) { return terms == 1 && nb <= 4 ? 3 : 1; }
+
+// Many rows (prompts): each of a block's four waves has NT tiles of its own and all walk the same tokens.  A wave's tile of 16 tokens (at
+// width 256 its keys or its values) is widened once for the block into LDS, in the order in which the matrix instructions take it: 64
+// tokens (32) at a time into one of two buffers while the other is read, one barrier for each.  A wave's next raw rows are requested as
+// soon as it has widened the last, a whole chunk ahead.
+template <int NB, int NT, int TERMS>
+__global__ __launch_bounds__(256, NB == 8 && TERMS == 3 ? 1 : 2) void k_kv_attend_wide(const KvAttendArgs a) {
+    constexpr uint32_t TILES = NB == 8 ? 2 : 4, T = 16 * TILES;
+    constexpr bool BOTH = NB < 8;  // a wave widens keys and values of its tile
+    __shared__ uint4 keys[2][TILES][NB][64], vals[2][TILES / 2][2 * NB][64];
+    const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4;
+    const KvBlock blk(a, 64 * NT);
+    if (blk.row0 >= blk.rows) return;
+    const uint32_t t0 = blk.split * a.split_tokens;
+    if (a.splits > 1 && t0 >= blk.end) return;
+    const uint32_t t1 = a.splits > 1 ? min(t0 + a.split_tokens, blk.end) : blk.end;
+    const uint32_t wave_row = blk.row0 + wave * (16 * NT);
+
+    KvRows<NB, NT, TERMS> r;
+    r.clear();
+    uint32_t limit[NT];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+        const uint32_t row = wave_row + t * 16 + (lane & 15);
+        limit[t] = row < blk.rows ? blk.limit(a, row) : 0;
+        r.load_q(t, blk.query(a, row, TERMS == 1 ? 2 : 4), a.g.dim);
+    }
+    const bool rows_here = wave_row < blk.rows;
+    const uint32_t all_see = rows_here ? __builtin_amdgcn_readfirstlane(blk.limit(a, wave_row)) : 0;
+    const uint32_t wave_end = rows_here ? min(t1, __builtin_amdgcn_readfirstlane(blk.limit(a, min(wave_row + 16 * NT, blk.rows) - 1))) : 0;
+    uint32_t seen_from = ~0u;
+
+    if (t0 < t1) {
+        const uint32_t half = a.g.page_size * 16 * NB, mask = a.g.page_size - 1;
+        const uint8_t *heads = a.cache + (uint64_t)blk.head * a.g.head_bytes;
+        KvPages pages(a, blk.i, t0, t1);
+        const uint32_t chunks = (t1 - t0 + T - 1) / T, tile = BOTH ? wave : wave & 1;
+        const bool does_keys = BOTH || wave < 2, does_vals = BOTH || wave >= 2;
+        const uint32_t key_at = (lane & 15) * (16 * NB) + g * (4 * NB), key_scale_at = (lane & 15) * NB, val_at = g * (64 * NB) + (lane & 15) * (4 * NB),
+                       val_scale_at = g * (4 * NB) + v_block<NB>(lane & 15) * 4;
+        uint32_t k[NB], v[BOTH ? NB : 1], ks = 0, vs = 0;  // raw rows of the chunk after the one that is read (v shares k at width 256)
+        uint32_t *const vv = BOTH ? v : k;
+        // bit x: page of the chunk's tile x is there
+        auto fetch = [&](uint32_t c) -> uint32_t {
+            c = min(c, chunks - 1);
+            pages.reach(c * TILES);
+            const uint32_t in = (t0 + c * T + 16 * tile) & mask;
+            const uint8_t *p = heads + pages.page(c * TILES + tile) * a.g.page_bytes, *kp = p + in * (16 * NB), *scales = p + 2 * half + in * NB;
+            if (does_keys) {
+                load_words<NB>(k, kp + key_at);
+                ks = load_key_scales<NB>(scales + key_scale_at, g);
+            }
+            if (does_vals) {
+                load_words<NB>(vv, kp + half + val_at);
+                vs = *reinterpret_cast<const uint32_t *>(scales + a.g.page_size * NB + val_scale_at);
+            }
+            return pages.there(c * TILES) & ((1u << TILES) - 1);
+        };
+        auto widen = [&](uint32_t c, uint32_t there) {
+            const uint32_t buf = c & 1, at = t0 + c * T + 16 * tile + 4 * g;
+            if (does_keys) {
+#pragma unroll
+                for (int b = 0; b < NB; ++b) keys[buf][tile][b][lane] = __builtin_bit_cast(uint4, widen_key(k[b], pow2_of(ks, NB == 8 ? b / 4 : 0)));
+            }
+            if (does_vals) {
+                uint32_t word = vs & live_scales(there >> tile & 1, at, t1);
+                float scale[4];
+                r.nan_at = min(r.nan_at, value_scales<1>(&word, scale, [&](int, int j) { return at + j; }));
+#pragma unroll
+                for (int b = 0; b < NB; ++b) {
+                    uint2 lo, hi;
+                    widen_values<NB>(vv, scale, b, lo, hi);
+                    reinterpret_cast<uint2 *>(&vals[buf][tile / 2][2 * b][lane])[tile & 1] = lo;
+                    reinterpret_cast<uint2 *>(&vals[buf][tile / 2][2 * b + 1][lane])[tile & 1] = hi;
+                }
+            }
+        };
+        uint32_t there = fetch(0);
+        widen(0, there);
+        uint32_t there_next = fetch(1);
+        for (uint32_t c = 0; c < chunks; ++c) {
+            __syncthreads();  // chunk c is whole; the buffer of chunk c + 1 has been read
+            const uint32_t t = t0 + c * T, buf = c & 1;
+            if (there) seen_from = min(seen_from, t + 16 * (uint32_t)__builtin_ctz(there));
+#pragma unroll
+            for (uint32_t h = 0; h < TILES / 2; ++h) {
+                const uint32_t th = t + 32 * h;
+                if (th >= wave_end) break;
+                const bool here[2] = {(there >> (2 * h) & 1) != 0, (there >> (2 * h + 1) & 1) != 0};
+                f32x4 s[NT][2];
+                r.scores(s, [&](int x, int b) { return __builtin_bit_cast(bf16x8, keys[buf][2 * h + x][b][lane]); });
+                bf16x8 p[NT][TERMS];
+                r.weights(s, p, a.scale_log2, !(here[0] && here[1]) || th + 32 > all_see || th + 32 > t1,
+                          [&](int row_tile, int x, int j) { const uint32_t at = th + 16 * x + 4 * g + j; return here[x] && at < limit[row_tile] && at < t1; });
+                r.products(p, [&](int b, bf16x8 *v2) {
+                    v2[0] = __builtin_bit_cast(bf16x8, vals[buf][h][2 * b][lane]);
+                    v2[1] = __builtin_bit_cast(bf16x8, vals[buf][h][2 * b + 1][lane]);
+                });
+            }
+            there = there_next;
+            if (c + 1 < chunks) {
+                widen(c + 1, there);
+                there_next = fetch(c + 2);
+            }
+        }
+    }
+    r.close();
+    // each wave knows the NaN blocks that it widened: the smallest index over the four
+    __syncthreads();
+    uint32_t *const nan = reinterpret_cast<uint32_t *>(&keys[0][0][0][0]);
+    nan[wave * 64 + lane] = r.nan_at;
+    __syncthreads();
+    if (!rows_here) return;
+    r.nan_at = min(min(nan[lane], nan[64 + lane]), min(nan[128 + lane], nan[192 + lane]));
+    store_rows(a, blk, r, limit, wave_row, seen_from);
 }
 
 // Joins the splits (at most 256) of a row, one block for a (row, head): a thread for each split's maximum and sum, then four columns and
@@ -672,11 +865,11 @@ template <int NB>
 static void launch_attend(const KvAttendArgs &a, const KvCut &c, uint32_t type, hipStream_t s) {
     const dim3 grid((uint32_t)c.blocks), block(256);
     if (type == ZVDB_KV_F32) {
-        if (c.wide) hipLaunchKernelGGL((k_kv_attend<NB, wide_tiles(NB, 3), 3, true>), grid, block, 0, s, a);
-        else hipLaunchKernelGGL((k_kv_attend<NB, 1, 3, false>), grid, block, 0, s, a);
+        if (c.wide) hipLaunchKernelGGL((k_kv_attend_wide<NB, wide_tiles(NB, 3), 3>), grid, block, 0, s, a);
+        else hipLaunchKernelGGL((k_kv_attend<NB, 3>), grid, block, 0, s, a);
     } else {
-        if (c.wide) hipLaunchKernelGGL((k_kv_attend<NB, wide_tiles(NB, 1), 1, true>), grid, block, 0, s, a);
-        else hipLaunchKernelGGL((k_kv_attend<NB, 1, 1, false>), grid, block, 0, s, a);
+        if (c.wide) hipLaunchKernelGGL((k_kv_attend_wide<NB, wide_tiles(NB, 1), 1>), grid, block, 0, s, a);
+        else hipLaunchKernelGGL((k_kv_attend<NB, 1>), grid, block, 0, s, a);
     }
 }
 
