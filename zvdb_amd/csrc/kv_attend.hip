@@ -742,58 +742,68 @@ __global__ __launch_bounds__(256) void k_kv_join(const KvAttendArgs a) {
 
 // ---- attention over selected rows ---------------------------------------------------------------------------------------
 
-// A block takes one request and key/value head: its list of ids is resolved to rows of the cache in LDS (a search's ids and counts
-// as zvdb_hip_search_*_dev writes them), then its four waves take 32 entries at a time.
+// A block takes one request and key/value head: its list of ids is resolved to places in the cache in LDS (a search's ids and counts
+// as zvdb_hip_search_*_dev writes them), then its four waves take 32 entries at a time.  A list of 100 is three dependent reads (ids,
+// pages, rows) and one chunk to a wave, so what counts is how many blocks a unit holds; a token's V lies in 16 pieces of four tokens
+// each, of which the other three are read for nothing.
 constexpr uint32_t kSelPass = 1024;  // entries resolved at a time
 
 template <int NB, int TERMS>
-__global__ __launch_bounds__(256) void k_kv_attend_selected(const KvAttendArgs a) {
-    __shared__ uint64_t rows_at[kSelPass];  // page << 8 | token in it; ~0: not there
+__global__ __launch_bounds__(256, NB == 8 && TERMS == 3 ? 1 : NB == 8 || TERMS == 3 ? 2 : 4) void k_kv_attend_selected(const KvAttendArgs a) {
+    constexpr uint64_t kNo = ~0ull;
+    __shared__ uint64_t places[kSelPass];  // bytes from the cache's start to the page's part of this head | token in the page << 48; kNo: not there
     const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4;
     const uint32_t head = blockIdx.x % a.g.heads, b = blockIdx.x / a.g.heads, i = b % a.n, tile = b / a.n;
-    const uint32_t qheads = a.g.heads * a.group, length = a.lengths[i];
-    const uint32_t reach = (uint32_t)min((uint64_t)length, (uint64_t)a.table_stride << a.g.page_shift);
     const uint64_t list = (uint64_t)head * a.n + i;
-    const uint32_t entries = min(a.counts ? a.counts[list] : a.k, a.k);
+    const uint64_t *ids = a.ids + list * a.k;
+    constexpr uint32_t AHEAD = kSelPass / 256;
+    uint64_t id[AHEAD];  // the first pass's, asked for before the count is known
+#pragma unroll
+    for (uint32_t x = 0; x < AHEAD; ++x) id[x] = threadIdx.x + 256 * x < a.k ? ids[threadIdx.x + 256 * x] : kNo;
+    const uint32_t entries = min(a.counts ? a.counts[list] : a.k, a.k), length = a.lengths[i];
+    const uint32_t reach = (uint32_t)min((uint64_t)length, (uint64_t)a.table_stride << a.g.page_shift);
+    const uint32_t qheads = a.g.heads * a.group, row = tile * 16 + (lane & 15);
     constexpr uint32_t kSize = TERMS == 1 ? 2 : 4;
-    const uint32_t row = tile * 16 + (lane & 15);
     KvRows<NB, 1, TERMS> r;
     r.clear();
-    r.load_q(0, row < a.group ? static_cast<const uint8_t *>(a.q) + ((uint64_t)i * a.q_stride + (uint64_t)(head * a.group + row) * a.g.dim) * kSize : nullptr, a.g.dim);
     const uint32_t half = a.g.page_size * 16 * NB, mask = a.g.page_size - 1;
-    const uint8_t *heads = a.cache + (uint64_t)head * a.g.head_bytes;
+    const uint8_t *cache = a.cache + (uint64_t)head * a.g.head_bytes;
     bool any = false;
     for (uint32_t e0 = 0; e0 < entries; e0 += kSelPass) {
         const uint32_t m = min(entries - e0, kSelPass);
-        if (e0) __syncthreads();
-        for (uint32_t e = threadIdx.x; e < kSelPass && e < ((m + 31) & ~31u); e += 256) {
-            uint64_t at = ~0ull;
-            const uint64_t id = e < m ? a.ids[list * a.k + e0 + e] : ~0ull;
-            if (id < reach) {
-                const uint32_t page = a.tables[(uint64_t)i * a.table_stride + (uint32_t)(id >> a.g.page_shift)];
-                if (page < a.g.pages) at = (uint64_t)page << 8 | (id & mask);
-            }
-            rows_at[e] = at;
+        if (e0) {
+            __syncthreads();
+#pragma unroll
+            for (uint32_t x = 0; x < AHEAD; ++x) id[x] = e0 + threadIdx.x + 256 * x < a.k ? ids[e0 + threadIdx.x + 256 * x] : kNo;
         }
+#pragma unroll
+        for (uint32_t x = 0; x < AHEAD; ++x) {
+            const uint32_t e = threadIdx.x + 256 * x;
+            uint64_t at = kNo;
+            if (e < m && id[x] < reach) {
+                const uint32_t page = a.tables[(uint64_t)i * a.table_stride + (uint32_t)(id[x] >> a.g.page_shift)];
+                if (page < a.g.pages) at = page * a.g.page_bytes | (id[x] & mask) << 48;
+            }
+            places[e] = at;
+        }
+        if (e0 == 0) r.load_q(0, row < a.group ? static_cast<const uint8_t *>(a.q) + ((uint64_t)i * a.q_stride + (uint64_t)(head * a.group + row) * a.g.dim) * kSize : nullptr, a.g.dim);
         __syncthreads();
         for (uint32_t e = wave * 32; e < m; e += 128) {
             KvRaw<NB> raw;
-            bool seen[8];
+            uint32_t seen = 0;
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
-                const uint64_t key = rows_at[e + 16 * x + (lane & 15)];
-                const uint32_t tok = (uint32_t)key & 0xFF;
-                const uint8_t *p = heads + (key == ~0ull ? 0 : (key >> 8) * a.g.page_bytes);
-                const uint32_t kt = key == ~0ull ? 0 : tok;
+                const uint64_t key = places[e + 16 * x + (lane & 15)] == kNo ? 0 : places[e + 16 * x + (lane & 15)];
+                const uint8_t *p = cache + (key & 0xFFFFFFFFFFFFull);
+                const uint32_t kt = (uint32_t)(key >> 48);
                 load_words<NB>(raw.k[x], p + kt * (16 * NB) + g * (4 * NB));
                 raw.ks[x] = load_key_scales<NB>(p + 2 * half + kt * NB, g);
                 raw.vs[x] = 0;
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    const uint64_t val = rows_at[e + 16 * x + 4 * g + j];
-                    seen[4 * x + j] = val != ~0ull;
-                    const uint32_t vt = val == ~0ull ? 0 : (uint32_t)val & 0xFF;
-                    const uint8_t *w = heads + (val == ~0ull ? 0 : (val >> 8) * a.g.page_bytes);
+                    const uint64_t there = places[e + 16 * x + 4 * g + j], val = there == kNo ? 0 : there;
+                    const uint32_t vt = (uint32_t)(val >> 48);
+                    const uint8_t *w = cache + (val & 0xFFFFFFFFFFFFull);
                     const uint8_t *piece = w + half + kv_v_offset<NB>(vt, lane & 15);
                     if constexpr (NB == 2) {
                         const uint32_t u = *reinterpret_cast<const uint16_t *>(piece);
@@ -805,17 +815,24 @@ __global__ __launch_bounds__(256) void k_kv_attend_selected(const KvAttendArgs a
                         load_words<2>(raw.v[x] + 2 * j, piece);
                     }
                     const uint32_t s = w[2 * half + a.g.page_size * NB + (vt >> 2) * (4 * NB) + v_block<NB>(lane & 15) * 4 + (vt & 3)];
-                    raw.vs[x] |= (val == ~0ull ? 0u : s) << (8 * j);
-                    any |= seen[4 * x + j];
+                    raw.vs[x] |= (there == kNo ? 0u : s) << (8 * j);
+                    seen |= there == kNo ? 0u : 1u << (4 * x + j);
                 }
             }
-            r.step(raw, a.scale_log2, true, [&](int, int x, int j) { return seen[4 * x + j]; }, [](int, int) { return 0u; });
+            any |= seen != 0;
+            r.step(raw, a.scale_log2, true, [&](int, int x, int j) { return seen >> (4 * x + j) & 1; }, [](int, int) { return 0u; });
         }
     }
     r.close();
-    const bool some = __syncthreads_or(any);
-    join_waves<NB, TERMS>(r);
-    if (wave != 0) return;
+    bool some;
+    if (entries <= 32) {  // the first wave had it all
+        if (wave != 0) return;
+        some = __any(any);
+    } else {
+        some = __syncthreads_or(any);
+        join_waves<NB, TERMS>(r);
+        if (wave != 0) return;
+    }
     uint32_t nan_first[4];
     nan_blocks<NB>(r.nan_at, nan_first);
     if (row >= a.group) return;
