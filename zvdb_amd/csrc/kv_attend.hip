@@ -344,44 +344,54 @@ __device__ inline uint32_t live_scales(bool there, uint32_t at, uint32_t t1) {
 
 __device__ inline float lse_of(float m, float l) { return (m + __log2f(l)) * kLn2; }
 
-// Joins the four waves of a block, each with its own tokens, in wave 0 (all 256 threads call this).  Sums in a fixed order.
-template <int NB, int TERMS>
-__device__ inline void join_waves(KvRows<NB, 1, TERMS> &r) {
-    __shared__ float ml[4][2][16];
-    __shared__ f32x4 buf[2][2 * NB][64];
-    __shared__ uint32_t nan[4][64];
-    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    if (lane < 16) { ml[wave][0][lane] = r.m[0]; ml[wave][1][lane] = r.l[0]; }
-    nan[wave][lane] = r.nan_at;
-    __syncthreads();
-    const uint32_t row = lane & 15;
-    const float m = fmaxf(fmaxf(ml[0][0][row], ml[1][0][row]), fmaxf(ml[2][0][row], ml[3][0][row]));
-    float l = 0;
+// Where the waves of a block that share 16 rows and have tokens of their own are joined: every wave leaves what it has, and after one
+// barrier all threads sum it, four columns each, in the waves' order.  (Rows are padded by four words against bank conflicts.)
+template <int NB, int WAVES>
+struct KvJoin {
+    float o[WAVES][16][32 * NB + 4], m[WAVES][16], l[WAVES][16];
+
+    // `rows` of the 16 and the first `waves` waves count (uniform); a NaN token below `limit` (this lane's row's) spoils its columns.  All
+    // threads call this.
+    template <int TERMS>
+    __device__ void leave(const KvRows<NB, 1, TERMS> &r, uint32_t rows, uint32_t waves, uint32_t limit) {
+        const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, row = lane & 15, g = lane >> 4;
+        uint32_t nan_first[4];
+        nan_blocks<NB>(r.nan_at, nan_first);
+        if (wave < waves && row < rows) {
 #pragma unroll
-    for (int w = 0; w < 4; ++w) l += ml[w][1][row] * __builtin_amdgcn_exp2f(ml[w][0][row] - m);
-    const float by = __builtin_amdgcn_exp2f(r.m[0] - m);
+            for (int x = 0; x < 4; ++x)
 #pragma unroll
-    for (int i = 0; i < 2 * NB; ++i) r.o[0][i] *= by;
-    if (wave >= 2)
-#pragma unroll
-        for (int i = 0; i < 2 * NB; ++i) buf[wave - 2][i][lane] = r.o[0][i];
-    __syncthreads();
-    if (wave < 2)
-#pragma unroll
-        for (int i = 0; i < 2 * NB; ++i) r.o[0][i] += buf[wave][i][lane];
-    __syncthreads();
-    if (wave == 1)
-#pragma unroll
-        for (int i = 0; i < 2 * NB; ++i) buf[0][i][lane] = r.o[0][i];
-    __syncthreads();
-    if (wave == 0) {
-#pragma unroll
-        for (int i = 0; i < 2 * NB; ++i) r.o[0][i] += buf[0][i][lane];
-        r.m[0] = m;
-        r.l[0] = l;
-        r.nan_at = min(min(nan[0][lane], nan[1][lane]), min(nan[2][lane], nan[3][lane]));
+                for (int e = 0; e < 2 * NB; e += 4) {
+                    float4 y = make_float4(r.o[0][e][x], r.o[0][e + 1][x], r.o[0][e + 2][x], r.o[0][e + 3][x]);
+                    if (nan_first[x] < limit) y.x = y.y = y.z = y.w = __uint_as_float(0x7FC00000u);
+                    *reinterpret_cast<float4 *>(&o[wave][row][(4 * g + x) * 2 * NB + e]) = y;
+                }
+            if (g == 0) { m[wave][row] = r.m[0]; l[wave][row] = r.l[0]; }
+        }
+        __syncthreads();
     }
-}
+
+    // emit(row, d, y[4], m, l) for four columns of every row
+    template <class Emit>
+    __device__ void take(uint32_t rows, uint32_t waves, uint32_t dim, Emit emit) const {
+        for (uint32_t item = threadIdx.x; item < rows * (8 * NB); item += 64 * WAVES) {
+            const uint32_t row = item / (8 * NB), d = item % (8 * NB) * 4;
+            if (d >= dim) continue;
+            float top = m[0][row], sum = 0, y[4] = {};
+#pragma unroll
+            for (int w = 1; w < WAVES; ++w) top = w < waves ? fmaxf(top, m[w][row]) : top;
+#pragma unroll
+            for (int w = 0; w < WAVES; ++w) {
+                if (w >= waves) break;
+                const float by = __builtin_amdgcn_exp2f(m[w][row] - top);
+                const float4 x = *reinterpret_cast<const float4 *>(&o[w][row][d]);
+                sum += l[w][row] * by;
+                y[0] += x.x * by; y[1] += x.y * by; y[2] += x.z * by; y[3] += x.w * by;
+            }
+            emit(row, d, y, top, sum);
+        }
+    }
+};
 
 // ---- attention over whole requests --------------------------------------------------------------------------------------
 
@@ -493,7 +503,7 @@ __global__ __launch_bounds__(256, NB == 8 && TERMS == 3 ? 1 : NB == 8 || TERMS =
     uint32_t t0 = blk.split * a.split_tokens;
     if (a.splits > 1 && t0 >= blk.end) return;  // (no row of the block sees a token of this split: k_kv_join knows)
     uint32_t t1 = a.splits > 1 ? min(t0 + a.split_tokens, blk.end) : blk.end;
-    const uint32_t quarter = ((t1 - t0 + 127) >> 7) << 5;  // this wave's, in whole chunks
+    const uint32_t part = t1 - t0, quarter = ((part + 127) >> 7) << 5;  // this wave's, in whole chunks
     t0 = min(t0 + wave * quarter, t1);
     t1 = min(t0 + quarter, t1);
 
@@ -547,11 +557,32 @@ __global__ __launch_bounds__(256, NB == 8 && TERMS == 3 ? 1 : NB == 8 || TERMS =
         }
     }
     r.close();
+    __shared__ KvJoin<NB, 4> join;
     __shared__ uint32_t from[4];
     if (lane == 0) from[wave] = seen_from;
-    join_waves<NB, TERMS>(r);
-    if (wave != 0) return;
-    store_rows(a, blk, r, &limit, blk.row0, min(min(from[0], from[1]), min(from[2], from[3])));
+    const uint32_t rows = min(blk.rows - blk.row0, 16u);
+    const uint32_t waves = quarter ? min((part + quarter - 1) / quarter, 4u) : 1;  // that have tokens
+    join.leave(r, rows, waves, limit);
+    seen_from = min(min(from[0], from[1]), min(from[2], from[3]));
+    const bool whole = a.splits == 1;
+    join.take(rows, waves, a.g.dim, [&](uint32_t row, uint32_t d, float *y, float m, float l) {
+        const uint64_t at = blk.place(a, blk.row0 + row);
+        const bool some = seen_from < blk.limit(a, blk.row0 + row);
+        if (whole) {
+            const float by = some ? 1.0f / l : 0.0f;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) y[e] *= by;
+            store_columns<2, TERMS>(static_cast<uint8_t *>(a.out) + at * a.g.dim * (TERMS == 1 ? 2 : 4), d, a.g.dim, y);
+            if (d == 0 && a.lse) a.lse[at] = some ? lse_of(m, l) : -INFINITY;
+        } else {
+            float *to = a.part + (at * a.splits + blk.split) * (a.g.dim + 4);
+            store_columns<2, 3>(to, d, a.g.dim, y);
+            if (d == 0) {
+                to[a.g.dim] = some ? m : -INFINITY;  // -inf: this split saw nothing
+                to[a.g.dim + 1] = l;
+            }
+        }
+    });
 }
 
 // Row tiles of a wave of k_kv_attend_wide: what 256 registers hold
@@ -751,7 +782,11 @@ constexpr uint32_t kSelPass = 1024;  // entries resolved at a time
 template <int NB, int TERMS>
 __global__ __launch_bounds__(256, NB == 8 && TERMS == 3 ? 1 : NB == 8 || TERMS == 3 ? 2 : 4) void k_kv_attend_selected(const KvAttendArgs a) {
     constexpr uint64_t kNo = ~0ull;
-    __shared__ uint64_t places[kSelPass];  // bytes from the cache's start to the page's part of this head | token in the page << 48; kNo: not there
+    __shared__ union {
+        uint64_t places[kSelPass];  // bytes from the cache's start to the page | token in the page << 48; kNo: not there
+        KvJoin<NB, 4> join;
+    } lds;
+    uint64_t *const places = lds.places;
     const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4;
     const uint32_t head = blockIdx.x % a.g.heads, b = blockIdx.x / a.g.heads, i = b % a.n, tile = b / a.n;
     const uint64_t list = (uint64_t)head * a.n + i;
@@ -824,28 +859,17 @@ __global__ __launch_bounds__(256, NB == 8 && TERMS == 3 ? 1 : NB == 8 || TERMS =
         }
     }
     r.close();
-    bool some;
-    if (entries <= 32) {  // the first wave had it all
-        if (wave != 0) return;
-        some = __any(any);
-    } else {
-        some = __syncthreads_or(any);
-        join_waves<NB, TERMS>(r);
-        if (wave != 0) return;
-    }
-    uint32_t nan_first[4];
-    nan_blocks<NB>(r.nan_at, nan_first);
-    if (row >= a.group) return;
-    const uint64_t out_row = (uint64_t)i * qheads + head * a.group + row;
-    const float by = some ? 1.0f / r.l[0] : 0.0f;
+    const bool some = __syncthreads_or(any);  // (and the places have been read)
+    const uint32_t rows = min(a.group - tile * 16, 16u), waves = min((entries + 31) / 32, 4u);
+    lds.join.leave(r, rows, waves ? waves : 1, 1);
+    lds.join.take(rows, waves ? waves : 1, a.g.dim, [&](uint32_t at, uint32_t d, float *y, float m, float l) {
+        const uint64_t out_row = (uint64_t)i * qheads + head * a.group + tile * 16 + at;
+        const float by = some ? 1.0f / l : 0.0f;
 #pragma unroll
-    for (int x = 0; x < 4; ++x) {
-        float y[2 * NB];
-#pragma unroll
-        for (int e = 0; e < 2 * NB; ++e) y[e] = nan_first[x] == 0 ? __uint_as_float(0x7FC00000u) : r.o[0][e][x] * by;
-        store_columns<NB, TERMS>(static_cast<uint8_t *>(a.out) + out_row * a.g.dim * kSize, (4 * g + x) * 2 * NB, a.g.dim, y);
-    }
-    if (g == 0 && a.lse) a.lse[out_row] = some ? lse_of(r.m[0], r.l[0]) : -INFINITY;
+        for (int e = 0; e < 4; ++e) y[e] *= by;
+        store_columns<2, TERMS>(static_cast<uint8_t *>(a.out) + out_row * a.g.dim * kSize, d, a.g.dim, y);
+        if (d == 0 && a.lse) a.lse[out_row] = some ? lse_of(m, l) : -INFINITY;
+    });
 }
 
 // ---- launches -----------------------------------------------------------------------------------------------------------
