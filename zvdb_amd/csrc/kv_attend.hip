@@ -65,12 +65,13 @@ __device__ inline void load_words(uint32_t *dst, const uint8_t *p) {
     }
 }
 
-// the scale bytes of the blocks that lane group g's part of a key row lies in: one byte, two at width 256
+// the scale bytes of the blocks that a lane group's part of a key row lies in: one byte, two at width 256
 template <int NB>
-__device__ inline uint32_t load_key_scales(const uint8_t *p, uint32_t g) {
-    if constexpr (NB == 8) return *reinterpret_cast<const uint16_t *>(p + 2 * g);
-    else return p[NB == 4 ? g : g / 2];
+__device__ inline uint32_t load_key_scales(const uint8_t *p) {
+    if constexpr (NB == 8) return *reinterpret_cast<const uint16_t *>(p);
+    else return *p;
 }
+__device__ inline uint32_t key_scale_of(uint32_t g, int nb) { return nb == 8 ? 2 * g : nb == 4 ? g : g / 2; }
 
 __device__ inline float pow2_of(uint32_t word, int byte) { return __uint_as_float(((word >> (8 * byte)) & 0xFFu) << 23); }
 
@@ -193,9 +194,9 @@ struct KvRows {
 #pragma unroll
         for (int t = 0; t < NT; ++t) s[t][0] = s[t][1] = f32x4{0, 0, 0, 0};
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
+        for (int b = 0; b < NB; ++b)
 #pragma unroll
-            for (int b = 0; b < NB; ++b) {
+            for (int i = 0; i < 2; ++i) {  // (the two token tiles in turn: sums that do not wait for each other)
                 const bf16x8 a = key(i, b);
 #pragma unroll
                 for (int t = 0; t < NT; ++t)
@@ -430,22 +431,26 @@ struct KvBlock {
     __device__ uint64_t place(const KvAttendArgs &a, uint32_t row) const { return (uint64_t)(first + row / a.group) * (a.g.heads * a.group) + head * a.group + row % a.group; }
 };
 
-// The pages of the tiles (16 tokens) from `t0` on, gone through in order: 64 of them lie in a register, one to a lane, and the next 64 are
-// on their way, so that no load of a page waits for its number.  (All 64 lanes call these; tiles behind the last page get the last.)
+// The pages of the tiles (16 tokens) from `t0` on, gone through in order: where 64 of them start lies in registers, one to a lane, and the
+// next 64 are on their way, so that no load of a page waits for its number or for a multiplication.  (All 64 lanes call these; tiles
+// behind the last page get the last.)
 struct KvPages {
     const uint32_t *table;
-    uint32_t t0, last, shift, pages, base, ids, next;
+    uint64_t page_bytes;
+    uint32_t t0, last, shift, pages, base, next, low, high;
     uint64_t are;
 
     __device__ KvPages(const KvAttendArgs &a, uint32_t request, uint32_t from, uint32_t to)
-        : table(a.tables + (uint64_t)request * a.table_stride), t0(from), last((to - 1) >> a.g.page_shift), shift(a.g.page_shift), pages(a.g.pages), base(0) {
+        : table(a.tables + (uint64_t)request * a.table_stride), page_bytes(a.g.page_bytes), t0(from), last((to - 1) >> a.g.page_shift), shift(a.g.page_shift), pages(a.g.pages), base(0) {
         next = read(0);
         take();
     }
     __device__ uint32_t read(uint32_t tile) const { return table[min((t0 + 16 * (tile + (threadIdx.x & 63))) >> shift, last)]; }
     __device__ void take() {
         are = __ballot(next < pages);
-        ids = next < pages ? next : 0;
+        const uint64_t at = (next < pages ? next : 0) * page_bytes;
+        low = (uint32_t)at;
+        high = (uint32_t)(at >> 32);
         next = read(base + 64);
     }
     __device__ void reach(uint32_t tile) {  // before anything is asked about the tiles from `tile` (uniform) to the next multiple of 64
@@ -454,8 +459,22 @@ struct KvPages {
             take();
         }
     }
-    __device__ uint32_t page(uint32_t tile) const { return __builtin_amdgcn_readlane(ids, tile - base); }  // 0 where there is none
-    __device__ uint32_t there(uint32_t tile) const { return (uint32_t)(are >> (tile - base)); }            // bit 0: the tile has a page; bit 1: the next; ...
+    // where the tile's page starts in the cache (the first page's place if it has none)
+    __device__ uint64_t start(uint32_t tile) const { return (uint64_t)(uint32_t)__builtin_amdgcn_readlane(high, tile - base) << 32 | (uint32_t)__builtin_amdgcn_readlane(low, tile - base); }
+    __device__ uint32_t there(uint32_t tile) const { return (uint32_t)(are >> (tile - base)); }  // bit 0: the tile has a page; bit 1: the next; ...
+};
+
+// What a lane adds to the place of a tile in its page: the parts that a tile's tokens (16 NB or NB bytes each) move are uniform
+template <int NB>
+struct KvLane {
+    uint32_t key, key_scale, value, value_scale;
+    __device__ KvLane(uint32_t half, uint32_t page_size) {
+        const uint32_t c = threadIdx.x & 15, g = (threadIdx.x & 63) >> 4;
+        key = c * (16 * NB) + g * (4 * NB);
+        key_scale = 2 * half + c * NB + key_scale_of(g, NB);
+        value = half + g * (64 * NB) + c * (4 * NB);
+        value_scale = 2 * half + page_size * NB + g * (4 * NB) + v_block<NB>(c) * 4;
+    }
 };
 
 // Writes a wave's rows: the result, or (several splits) the part that k_kv_join joins
@@ -519,20 +538,17 @@ __global__ __launch_bounds__(256, NB == 8 && TERMS == 3 ? 1 : NB == 8 || TERMS =
         const uint8_t *heads = a.cache + (uint64_t)blk.head * a.g.head_bytes;
         const uint32_t chunks = (t1 - t0 + 31) >> 5;
         KvPages pages(a, blk.i, t0, t1);
-        // what a lane adds to a tile's place: the rest of an address is uniform
-        const uint32_t key_at = (lane & 15) * (16 * NB) + g * (4 * NB), key_scale_at = (lane & 15) * NB, val_at = g * (64 * NB) + (lane & 15) * (4 * NB),
-                       val_scale_at = g * (4 * NB) + v_block<NB>(lane & 15) * 4;
+        const KvLane<NB> at(half, a.g.page_size);
         auto load = [&](KvRaw<NB> &raw, uint32_t c) -> uint32_t {
             pages.reach(2 * c);
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
-                const uint8_t *p = heads + pages.page(2 * c + x) * a.g.page_bytes;
+                const uint8_t *p = heads + pages.start(2 * c + x);
                 const uint32_t in = (t0 + 32 * c + 16 * x) & mask;
-                const uint8_t *keys = p + in * (16 * NB), *vals = keys + half, *scales = p + 2 * half + in * NB;
-                load_words<NB>(raw.k[x], keys + key_at);
-                raw.ks[x] = load_key_scales<NB>(scales + key_scale_at, g);
-                load_words<NB>(raw.v[x], vals + val_at);
-                raw.vs[x] = *reinterpret_cast<const uint32_t *>(scales + a.g.page_size * NB + val_scale_at);
+                load_words<NB>(raw.k[x], p + (at.key + in * (16 * NB)));
+                raw.ks[x] = load_key_scales<NB>(p + (at.key_scale + in * NB));
+                load_words<NB>(raw.v[x], p + (at.value + in * (16 * NB)));
+                raw.vs[x] = *reinterpret_cast<const uint32_t *>(p + (at.value_scale + in * NB));
             }
             return pages.there(2 * c) & 3;
         };
@@ -625,8 +641,7 @@ __global__ __launch_bounds__(256, NB == 8 && TERMS == 3 ? 1 : 2) void k_kv_atten
         KvPages pages(a, blk.i, t0, t1);
         const uint32_t chunks = (t1 - t0 + T - 1) / T, tile = BOTH ? wave : wave & 1;
         const bool does_keys = BOTH || wave < 2, does_vals = BOTH || wave >= 2;
-        const uint32_t key_at = (lane & 15) * (16 * NB) + g * (4 * NB), key_scale_at = (lane & 15) * NB, val_at = g * (64 * NB) + (lane & 15) * (4 * NB),
-                       val_scale_at = g * (4 * NB) + v_block<NB>(lane & 15) * 4;
+        const KvLane<NB> place(half, a.g.page_size);
         uint32_t k[NB], v[BOTH ? NB : 1], ks = 0, vs = 0;  // raw rows of the chunk after the one that is read (v shares k at width 256)
         uint32_t *const vv = BOTH ? v : k;
         // bit x: page of the chunk's tile x is there
@@ -634,14 +649,14 @@ __global__ __launch_bounds__(256, NB == 8 && TERMS == 3 ? 1 : 2) void k_kv_atten
             c = min(c, chunks - 1);
             pages.reach(c * TILES);
             const uint32_t in = (t0 + c * T + 16 * tile) & mask;
-            const uint8_t *p = heads + pages.page(c * TILES + tile) * a.g.page_bytes, *kp = p + in * (16 * NB), *scales = p + 2 * half + in * NB;
+            const uint8_t *p = heads + pages.start(c * TILES + tile);
             if (does_keys) {
-                load_words<NB>(k, kp + key_at);
-                ks = load_key_scales<NB>(scales + key_scale_at, g);
+                load_words<NB>(k, p + (place.key + in * (16 * NB)));
+                ks = load_key_scales<NB>(p + (place.key_scale + in * NB));
             }
             if (does_vals) {
-                load_words<NB>(vv, kp + half + val_at);
-                vs = *reinterpret_cast<const uint32_t *>(scales + a.g.page_size * NB + val_scale_at);
+                load_words<NB>(vv, p + (place.value + in * (16 * NB)));
+                vs = *reinterpret_cast<const uint32_t *>(p + (place.value_scale + in * NB));
             }
             return pages.there(c * TILES) & ((1u << TILES) - 1);
         };
@@ -832,7 +847,7 @@ __global__ __launch_bounds__(256, NB == 8 && TERMS == 3 ? 1 : NB == 8 || TERMS =
                 const uint8_t *p = cache + (key & 0xFFFFFFFFFFFFull);
                 const uint32_t kt = (uint32_t)(key >> 48);
                 load_words<NB>(raw.k[x], p + kt * (16 * NB) + g * (4 * NB));
-                raw.ks[x] = load_key_scales<NB>(p + 2 * half + kt * NB, g);
+                raw.ks[x] = load_key_scales<NB>(p + 2 * half + kt * NB + key_scale_of(g, NB));
                 raw.vs[x] = 0;
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
