@@ -400,15 +400,21 @@ struct KvJoin {
 // numbered head first, so that (with 8 heads) an XCD's L2 keeps the pages of its own heads, and row tiles last to first, so that the
 // causal ones with most tokens start first.  The requests turn by one from one tile or split to the next: blocks are dealt to the shader
 // engines in order, and without it one of them gets all of a long request (4 prompts: 465 -> 331 us).
-struct KvBlock {
-    uint32_t head, i, split, first, count, length, reach, rows, row0, end;
-
-    __device__ KvBlock(const KvAttendArgs &a, uint32_t block_rows) {
+struct KvWhere {  // what the block's number says: known before anything is read
+    uint32_t head, i, split, tile;
+    __device__ explicit KvWhere(const KvAttendArgs &a) {
         const uint32_t b = blockIdx.x / a.g.heads, turn = b / a.n;
         head = blockIdx.x % a.g.heads;
         i = (b + turn) % a.n;
         split = turn % a.splits;
-        row0 = (a.tiles - 1 - turn / a.splits) * block_rows;
+        tile = a.tiles - 1 - turn / a.splits;
+    }
+};
+struct KvBlock : KvWhere {
+    uint32_t first, count, length, reach, rows, row0, end;
+
+    __device__ KvBlock(const KvAttendArgs &a, const KvWhere &where, uint32_t block_rows) : KvWhere(where) {
+        row0 = tile * block_rows;
         // rows [first, first + count) of q, `length` tokens, of which those below `reach` can be read
         first = min(a.starts[i], a.rows);
         const uint32_t next = min(a.starts[i + 1], a.rows);
@@ -431,22 +437,26 @@ struct KvBlock {
     __device__ uint64_t place(const KvAttendArgs &a, uint32_t row) const { return (uint64_t)(first + row / a.group) * (a.g.heads * a.group) + head * a.group + row % a.group; }
 };
 
-// The pages of the tiles (16 tokens) from `t0` on, gone through in order: where 64 of them start lies in registers, one to a lane, and the
-// next 64 are on their way, so that no load of a page waits for its number or for a multiplication.  (All 64 lanes call these; tiles
-// behind the last page get the last.)
+// The pages of a wave's tiles (16 tokens), gone through in order: where 64 of them start lies in registers, one to a lane, and the next 64
+// are on their way, so that no load of a page waits for its number or for a multiplication.  The wave takes STEP tokens of every STRIDE
+// from `t0` on.  Entries behind the request's own are read too, and are nothing to anybody: their tokens are not seen.  (All 64 lanes
+// call these.)
+template <uint32_t STEP, uint32_t STRIDE>
 struct KvPages {
     const uint32_t *table;
     uint64_t page_bytes;
     uint32_t t0, last, shift, pages, base, next, low, high;
     uint64_t are;
 
-    __device__ KvPages(const KvAttendArgs &a, uint32_t request, uint32_t from, uint32_t to)
-        : table(a.tables + (uint64_t)request * a.table_stride), page_bytes(a.g.page_bytes), t0(from), last((to - 1) >> a.g.page_shift), shift(a.g.page_shift), pages(a.g.pages), base(0) {
+    __device__ KvPages(const KvAttendArgs &a, uint32_t request, uint32_t from)
+        : table(a.tables + (uint64_t)request * a.table_stride), page_bytes(a.g.page_bytes), t0(from), last(a.table_stride - 1), shift(a.g.page_shift), pages(a.g.pages), base(0) {
         next = read(0);
-        take();
     }
-    __device__ uint32_t read(uint32_t tile) const { return table[min((t0 + 16 * (tile + (threadIdx.x & 63))) >> shift, last)]; }
-    __device__ void take() {
+    __device__ uint32_t read(uint32_t tile) const {
+        const uint32_t at = tile + (threadIdx.x & 63);
+        return table[min((t0 + at / (STEP / 16) * STRIDE + at % (STEP / 16) * 16) >> shift, last)];
+    }
+    __device__ void take() {  // once before the first tile is asked for
         are = __ballot(next < pages);
         const uint64_t at = (next < pages ? next : 0) * page_bytes;
         low = (uint32_t)at;
@@ -512,19 +522,18 @@ __device__ inline void store_rows(const KvAttendArgs &a, const KvBlock &blk, con
     }
 }
 
-// Few rows (decode): 16 of them to a block, whose four waves divide the split's tokens and are joined in LDS.  Each wave widens what it
+// Few rows (decode): 16 of them to a block, whose four waves take every fourth chunk of the split's tokens and are joined in LDS.  Each wave widens what it
 // loads, one chunk of 32 tokens ahead.
 template <int NB, int TERMS>
 __global__ __launch_bounds__(256, NB == 8 && TERMS == 3 ? 1 : NB == 8 || TERMS == 3 ? 2 : NB == 4 ? 3 : 4) void k_kv_attend(const KvAttendArgs a) {
     const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4;
-    const KvBlock blk(a, 16);
+    const KvWhere where(a);
+    const uint32_t from = where.split * a.split_tokens, t0 = from + 32 * wave;  // this wave's chunks: every fourth
+    KvPages<32, 128> pages(a, where.i, t0);                                     // (on their way together with the lengths)
+    const KvBlock blk(a, where, 16);
     if (blk.row0 >= blk.rows) return;
-    uint32_t t0 = blk.split * a.split_tokens;
-    if (a.splits > 1 && t0 >= blk.end) return;  // (no row of the block sees a token of this split: k_kv_join knows)
-    uint32_t t1 = a.splits > 1 ? min(t0 + a.split_tokens, blk.end) : blk.end;
-    const uint32_t part = t1 - t0, quarter = ((part + 127) >> 7) << 5;  // this wave's, in whole chunks
-    t0 = min(t0 + wave * quarter, t1);
-    t1 = min(t0 + quarter, t1);
+    if (a.splits > 1 && from >= blk.end) return;  // (no row of the block sees a token of this split: k_kv_join knows)
+    const uint32_t t1 = a.splits > 1 ? min(from + a.split_tokens, blk.end) : blk.end;
 
     KvRows<NB, 1, TERMS> r;
     r.clear();
@@ -536,15 +545,15 @@ __global__ __launch_bounds__(256, NB == 8 && TERMS == 3 ? 1 : NB == 8 || TERMS =
     if (t0 < t1) {
         const uint32_t half = a.g.page_size * 16 * NB, mask = a.g.page_size - 1;
         const uint8_t *heads = a.cache + (uint64_t)blk.head * a.g.head_bytes;
-        const uint32_t chunks = (t1 - t0 + 31) >> 5;
-        KvPages pages(a, blk.i, t0, t1);
+        const uint32_t chunks = (t1 - t0 + 127) >> 7;
+        pages.take();
         const KvLane<NB> at(half, a.g.page_size);
         auto load = [&](KvRaw<NB> &raw, uint32_t c) -> uint32_t {
             pages.reach(2 * c);
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
                 const uint8_t *p = heads + pages.start(2 * c + x);
-                const uint32_t in = (t0 + 32 * c + 16 * x) & mask;
+                const uint32_t in = (t0 + 128 * c + 16 * x) & mask;
                 load_words<NB>(raw.k[x], p + (at.key + in * (16 * NB)));
                 raw.ks[x] = load_key_scales<NB>(p + (at.key_scale + in * NB));
                 load_words<NB>(raw.v[x], p + (at.value + in * (16 * NB)));
@@ -567,19 +576,19 @@ __global__ __launch_bounds__(256, NB == 8 && TERMS == 3 ? 1 : NB == 8 || TERMS =
         uint32_t there = load(cur, 0);
         for (uint32_t c = 0; c < chunks; ++c) {
             const uint32_t there_next = load(nxt, min(c + 1, chunks - 1));
-            work(cur, t0 + c * 32, there);
+            work(cur, t0 + c * 128, there);
             cur = nxt;
             there = there_next;
         }
     }
     r.close();
     __shared__ KvJoin<NB, 4> join;
-    __shared__ uint32_t from[4];
-    if (lane == 0) from[wave] = seen_from;
+    __shared__ uint32_t seen[4];
+    if (lane == 0) seen[wave] = seen_from;
     const uint32_t rows = min(blk.rows - blk.row0, 16u);
-    const uint32_t waves = quarter ? min((part + quarter - 1) / quarter, 4u) : 1;  // that have tokens
+    const uint32_t waves = t1 > from ? min((t1 - from + 31) / 32, 4u) : 1;  // that have tokens
     join.leave(r, rows, waves, limit);
-    seen_from = min(min(from[0], from[1]), min(from[2], from[3]));
+    seen_from = min(min(seen[0], seen[1]), min(seen[2], seen[3]));
     const bool whole = a.splits == 1;
     join.take(rows, waves, a.g.dim, [&](uint32_t row, uint32_t d, float *y, float m, float l) {
         const uint64_t at = blk.place(a, blk.row0 + row);
@@ -614,9 +623,11 @@ __global__ __launch_bounds__(256, NB == 8 && TERMS == 3 ? 1 : 2) void k_kv_atten
     constexpr bool BOTH = NB < 8;  // a wave widens keys and values of its tile
     __shared__ uint4 keys[2][TILES][NB][64], vals[2][TILES / 2][2 * NB][64];
     const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4;
-    const KvBlock blk(a, 64 * NT);
+    const KvWhere where(a);
+    const uint32_t t0 = where.split * a.split_tokens;
+    KvPages<T, T> pages(a, where.i, t0);
+    const KvBlock blk(a, where, 64 * NT);
     if (blk.row0 >= blk.rows) return;
-    const uint32_t t0 = blk.split * a.split_tokens;
     if (a.splits > 1 && t0 >= blk.end) return;
     const uint32_t t1 = a.splits > 1 ? min(t0 + a.split_tokens, blk.end) : blk.end;
     const uint32_t wave_row = blk.row0 + wave * (16 * NT);
@@ -638,7 +649,7 @@ __global__ __launch_bounds__(256, NB == 8 && TERMS == 3 ? 1 : 2) void k_kv_atten
     if (t0 < t1) {
         const uint32_t half = a.g.page_size * 16 * NB, mask = a.g.page_size - 1;
         const uint8_t *heads = a.cache + (uint64_t)blk.head * a.g.head_bytes;
-        KvPages pages(a, blk.i, t0, t1);
+        pages.take();
         const uint32_t chunks = (t1 - t0 + T - 1) / T, tile = BOTH ? wave : wave & 1;
         const bool does_keys = BOTH || wave < 2, does_vals = BOTH || wave >= 2;
         const KvLane<NB> place(half, a.g.page_size);
