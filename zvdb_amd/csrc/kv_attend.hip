@@ -522,14 +522,15 @@ __device__ inline void store_rows(const KvAttendArgs &a, const KvBlock &blk, con
     }
 }
 
-// Few rows (decode): 16 of them to a block, whose four waves take every fourth chunk of the split's tokens and are joined in LDS.  Each wave widens what it
-// loads, one chunk of 32 tokens ahead.
-template <int NB, int TERMS>
-__global__ __launch_bounds__(256, NB == 8 && TERMS == 3 ? 1 : NB == 8 || TERMS == 3 ? 2 : NB == 4 ? 3 : 4) void k_kv_attend(const KvAttendArgs a) {
+// Few rows (decode): 16 of them to a block, whose waves take the chunks of the split's tokens in turn and are joined in LDS.  Each wave
+// widens what it loads, one chunk of 32 tokens ahead.
+template <int NB, int TERMS, int WAVES>
+__global__ __launch_bounds__(64 * WAVES, NB == 8 && TERMS == 3 ? 1 : NB == 8 || TERMS == 3 || WAVES == 8 ? 2 : NB == 4 ? 3 : 4) void k_kv_attend(const KvAttendArgs a) {
+    constexpr uint32_t STRIDE = 32 * WAVES;
     const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4;
     const KvWhere where(a);
-    const uint32_t from = where.split * a.split_tokens, t0 = from + 32 * wave;  // this wave's chunks: every fourth
-    KvPages<32, 128> pages(a, where.i, t0);                                     // (on their way together with the lengths)
+    const uint32_t from = where.split * a.split_tokens, t0 = from + 32 * wave;  // the chunks of 32 go round the waves
+    KvPages<32, STRIDE> pages(a, where.i, t0);                                     // (on their way together with the lengths)
     const KvBlock blk(a, where, 16);
     if (blk.row0 >= blk.rows) return;
     if (a.splits > 1 && from >= blk.end) return;  // (no row of the block sees a token of this split: k_kv_join knows)
@@ -545,7 +546,7 @@ __global__ __launch_bounds__(256, NB == 8 && TERMS == 3 ? 1 : NB == 8 || TERMS =
     if (t0 < t1) {
         const uint32_t half = a.g.page_size * 16 * NB, mask = a.g.page_size - 1;
         const uint8_t *heads = a.cache + (uint64_t)blk.head * a.g.head_bytes;
-        const uint32_t chunks = (t1 - t0 + 127) >> 7;
+        const uint32_t chunks = (t1 - t0 + STRIDE - 1) / STRIDE;
         pages.take();
         const KvLane<NB> at(half, a.g.page_size);
         auto load = [&](KvRaw<NB> &raw, uint32_t c) -> uint32_t {
@@ -553,7 +554,7 @@ __global__ __launch_bounds__(256, NB == 8 && TERMS == 3 ? 1 : NB == 8 || TERMS =
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
                 const uint8_t *p = heads + pages.start(2 * c + x);
-                const uint32_t in = (t0 + 128 * c + 16 * x) & mask;
+                const uint32_t in = (t0 + STRIDE * c + 16 * x) & mask;
                 load_words<NB>(raw.k[x], p + (at.key + in * (16 * NB)));
                 raw.ks[x] = load_key_scales<NB>(p + (at.key_scale + in * NB));
                 load_words<NB>(raw.v[x], p + (at.value + in * (16 * NB)));
@@ -576,19 +577,20 @@ __global__ __launch_bounds__(256, NB == 8 && TERMS == 3 ? 1 : NB == 8 || TERMS =
         uint32_t there = load(cur, 0);
         for (uint32_t c = 0; c < chunks; ++c) {
             const uint32_t there_next = load(nxt, min(c + 1, chunks - 1));
-            work(cur, t0 + c * 128, there);
+            work(cur, t0 + c * STRIDE, there);
             cur = nxt;
             there = there_next;
         }
     }
     r.close();
-    __shared__ KvJoin<NB, 4> join;
-    __shared__ uint32_t seen[4];
+    __shared__ KvJoin<NB, WAVES> join;
+    __shared__ uint32_t seen[WAVES];
     if (lane == 0) seen[wave] = seen_from;
     const uint32_t rows = min(blk.rows - blk.row0, 16u);
-    const uint32_t waves = t1 > from ? min((t1 - from + 31) / 32, 4u) : 1;  // that have tokens
+    const uint32_t waves = t1 > from ? min((t1 - from + 31) / 32, (uint32_t)WAVES) : 1;  // that have tokens
     join.leave(r, rows, waves, limit);
-    seen_from = min(min(seen[0], seen[1]), min(seen[2], seen[3]));
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) seen_from = min(seen_from, seen[w]);
     const bool whole = a.splits == 1;
     join.take(rows, waves, a.g.dim, [&](uint32_t row, uint32_t d, float *y, float m, float l) {
         const uint64_t at = blk.place(a, blk.row0 + row);
@@ -777,7 +779,7 @@ __global__ __launch_bounds__(256) void k_kv_join(const KvAttendArgs a) {
 #pragma unroll
         for (uint32_t u = 0; u < AHEAD; ++u)
             if (lane + u * LANES < live) add(ahead[u], lane + u * LANES);
-#pragma unroll 4
+#pragma unroll 8
         for (uint32_t s = lane + AHEAD * LANES; s < live; s += LANES) add(*reinterpret_cast<const float4 *>(part + s * step + d), s);
     }
     sum[lane][tid % COLS] = o;
@@ -901,10 +903,14 @@ __global__ __launch_bounds__(256, NB == 8 && TERMS == 3 ? 1 : NB == 8 || TERMS =
 // ---- launches -----------------------------------------------------------------------------------------------------------
 
 // How a call is cut.  Rows of one (request, head) that fit 64 are few: blocks of 16 whose waves divide the tokens; more of them give
-// each wave its own tiles.  The tokens are split until the card has work for all its units, in parts of whole chunks.
+// each wave its own tiles.  Tokens are split until the card has four blocks for each unit: requests differ in length, so a good third of
+// the splits is empty.  Each part costs its start (some 5 us of dependent reads) and its place in the join: parts of few rows hold at
+// least 1,024 tokens (48 requests to 8,192 tokens: 2 / 3 / 5 splits 58.5 / 54.4 / 59.8 us; one of 32,768: 32 / 256 splits 15.5 / 28.9), and
+// two blocks a unit are left whole (64 requests of 2,048: 29.8 us, 39.8 with two splits).  Where even that leaves units empty a block
+// has eight waves (one request of 1,024 tokens: 9.6 us, 12.8 with four waves and splits).
 struct KvCut {
     bool wide;
-    uint32_t nt, tiles, splits, split_tokens;
+    uint32_t nt, tiles, splits, split_tokens, waves;
     uint64_t blocks;
 };
 
@@ -917,27 +923,30 @@ static KvCut kv_cut(const KvGeom &g, uint32_t type, uint32_t group, uint32_t n, 
     const uint32_t block_rows = c.wide ? 64 * c.nt : 16;
     c.tiles = (uint32_t)((rows + block_rows - 1) / block_rows);
     const uint64_t base = (uint64_t)g.heads * n * c.tiles;
-    const uint64_t want = (uint64_t)cus * (c.wide ? 4 : 8);  // blocks the card should have
-    uint64_t splits = base ? (want + base - 1) / base : 1;
-    const uint32_t least = c.wide ? 256 : 128;
+    const uint64_t want = (uint64_t)cus * 4;
+    uint64_t splits = base && (c.wide || base < 2 * (uint64_t)cus) ? (want + base - 1) / base : 1;
+    const uint32_t least = c.wide ? 256 : 1024;
     splits = std::min<uint64_t>(splits, ((uint64_t)max_length + least - 1) / least);
     splits = std::max<uint64_t>(std::min<uint64_t>(splits, 256), 1);
     c.split_tokens = (uint32_t)std::max<uint64_t>((((uint64_t)max_length + splits - 1) / splits + 127) / 128 * 128, 128);
     c.splits = (uint32_t)std::max<uint64_t>(((uint64_t)max_length + c.split_tokens - 1) / c.split_tokens, 1);
     c.blocks = base * c.splits;
+    c.waves = !c.wide && c.blocks <= (uint64_t)cus && w <= 128 && c.split_tokens > 256 ? 8 : 4;
     return c;
+}
+
+template <int NB, int TERMS>
+static void launch_attend_as(const KvAttendArgs &a, const KvCut &c, hipStream_t s) {
+    const dim3 grid((uint32_t)c.blocks), block(64 * c.waves);
+    if (c.wide) hipLaunchKernelGGL((k_kv_attend_wide<NB, wide_tiles(NB, TERMS), TERMS>), grid, block, 0, s, a);
+    else if (c.waves == 8) hipLaunchKernelGGL((k_kv_attend<NB < 8 ? NB : 4, TERMS, 8>), grid, block, 0, s, a);
+    else hipLaunchKernelGGL((k_kv_attend<NB, TERMS, 4>), grid, block, 0, s, a);
 }
 
 template <int NB>
 static void launch_attend(const KvAttendArgs &a, const KvCut &c, uint32_t type, hipStream_t s) {
-    const dim3 grid((uint32_t)c.blocks), block(256);
-    if (type == ZVDB_KV_F32) {
-        if (c.wide) hipLaunchKernelGGL((k_kv_attend_wide<NB, wide_tiles(NB, 3), 3>), grid, block, 0, s, a);
-        else hipLaunchKernelGGL((k_kv_attend<NB, 3>), grid, block, 0, s, a);
-    } else {
-        if (c.wide) hipLaunchKernelGGL((k_kv_attend_wide<NB, wide_tiles(NB, 1), 1>), grid, block, 0, s, a);
-        else hipLaunchKernelGGL((k_kv_attend<NB, 1>), grid, block, 0, s, a);
-    }
+    if (type == ZVDB_KV_F32) launch_attend_as<NB, 3>(a, c, s);
+    else launch_attend_as<NB, 1>(a, c, s);
 }
 
 template <int W>
