@@ -53,7 +53,7 @@ inline bool kv_aligned(const void *p, uintptr_t a) { return reinterpret_cast<uin
 #if defined(__HIPCC__)
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
-typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 // Offset of element `piece` of token t's V codes within a head's V region: 16 pieces of 2 NB elements, four tokens side by side

