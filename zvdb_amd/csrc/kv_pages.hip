@@ -76,57 +76,80 @@ __device__ inline uint32_t kv_owner(const uint32_t *first, uint32_t n, uint32_t 
     return lo;
 }
 
+// Sums of counts that stop at 2^31 - 1, which no call may reach: they saturate, so the order of the additions does not matter
+constexpr uint32_t kPlanFull = 0x7FFFFFFF;
+__device__ inline uint32_t sat_add(uint32_t a, uint32_t b) { return min(a + b, kPlanFull); }
+
+// Inclusive sums over 16 lanes (a DPP row), and from there over 64: no LDS
+template <int CTRL, int ROWS>
+__device__ inline uint32_t dpp_or_zero(uint32_t x) { return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, ROWS, 0xF, false); }
+__device__ inline uint32_t sum_upto_16(uint32_t x) {
+    x = sat_add(x, dpp_or_zero<0x111, 0xF>(x));  // row_shr:1
+    x = sat_add(x, dpp_or_zero<0x112, 0xF>(x));  // row_shr:2
+    x = sat_add(x, dpp_or_zero<0x114, 0xF>(x));  // row_shr:4
+    return sat_add(x, dpp_or_zero<0x118, 0xF>(x));  // row_shr:8
+}
+__device__ inline uint32_t sum_upto_64(uint32_t x) {
+    x = sum_upto_16(x);
+    x = sat_add(x, dpp_or_zero<0x142, 0xA>(x));  // row_bcast:15 into rows 1 and 3
+    return sat_add(x, dpp_or_zero<0x143, 0xC>(x));  // row_bcast:31 into rows 2 and 3
+}
+
 // Every block sums the whole batch (8 n bytes that stay in L2): one launch, no block waits for another, and nothing that a block
 // reads is written by one (a partly filled page's table entry is an older call's; new pages are read from the ring).  The unit of
 // work behind the sums is a RUN, the new tokens of one page: 16 lanes find its request -- a search over the threads' sums in LDS, then
 // a scan of that thread's at most 16 requests -- look its page up once and write its slots side by side.  Bound by latency: the sums
-// and one run are some ten dependent reads (2,048 prompts, 1.05M tokens: 16.1 us with a search for each token).
+// and one run are some ten dependent reads (2,048 prompts, 1.05M tokens: 10.0 us; 16.1 with a search for each token, 13.0 with sums in
+// 64 bits through LDS).
 __global__ __launch_bounds__(1024) void k_kv_plan(const KvPlanArgs a) {
     __shared__ uint32_t tok[1025], pag[1025], run[1025];  // sums before each thread's requests
-    __shared__ uint64_t wt[16], wp[16];
-    __shared__ uint32_t wr[16], bad;
+    __shared__ uint32_t wave_sum[3][16], bad;
     const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, nt = blockDim.x;
     const uint32_t per = (a.n + nt - 1) / nt, i0 = min(tid * per, a.n), i1 = min(i0 + per, a.n);
     const uint32_t mask = (1u << a.page_shift) - 1;
     if (tid == 0) bad = 0;
     __syncthreads();
-    uint64_t st = 0, sp = 0;
-    uint32_t sr = 0;
+    uint32_t st = 0, sp = 0, sr = 0;
     for (uint32_t i = i0; i < i1; ++i) {
-        const uint64_t c = a.lengths[i], e = c + a.fresh[i];
-        const uint64_t have = (c + mask) >> a.page_shift, want = (e + mask) >> a.page_shift;
-        if (want > a.table_stride || e > 0x7FFFFFFFull) bad = 1;  // (every writer writes the same)
-        st += e - c;
-        sp += want - have;
-        sr += e > c ? (uint32_t)(want - (c >> a.page_shift)) : 0;
+        const uint32_t c = a.lengths[i], f = a.fresh[i];
+        const uint64_t e = (uint64_t)c + f, want = (e + mask) >> a.page_shift;
+        if (want > a.table_stride || e > kPlanFull) {
+            bad = 1;  // (every writer writes the same)
+            st = sat_add(st, min(f, kPlanFull));
+            sp = sat_add(sp, (uint32_t)(want - (((uint64_t)c + mask) >> a.page_shift)));
+        } else {
+            st = sat_add(st, f);
+            sp = sat_add(sp, (uint32_t)want - ((c + mask) >> a.page_shift));
+            sr += f ? (uint32_t)want - (c >> a.page_shift) : 0;
+        }
     }
-    uint64_t it = st, ip = sp;  // inclusive scan over the block's threads
-    uint32_t ir = sr;
-    for (int d = 1; d < 64; d <<= 1) {
-        const uint64_t t = __shfl_up(it, d), p = __shfl_up(ip, d);
-        const uint32_t r = __shfl_up(ir, d);
-        if (lane >= (uint32_t)d) { it += t; ip += p; ir += r; }
-    }
-    if (lane == 63) { wt[wave] = it; wp[wave] = ip; wr[wave] = ir; }
+    uint32_t it = sum_upto_64(st), ip = sum_upto_64(sp), ir = sum_upto_64(sr);  // over the block's threads
+    if (lane == 63) { wave_sum[0][wave] = it; wave_sum[1][wave] = ip; wave_sum[2][wave] = ir; }
     __syncthreads();
-    uint64_t tt = 0, tp = 0;
-    uint32_t tr = 0;
-    for (uint32_t w = 0; w < nt / 64; ++w) {
-        if (w == wave) { it += tt; ip += tp; ir += tr; }
-        tt += wt[w];
-        tp += wp[w];
-        tr += wr[w];
+    uint32_t tt = 0, tp = 0, tr = 0;
+    {
+        const bool there = lane < nt / 64;
+        const uint32_t x = sum_upto_16(there ? wave_sum[0][lane & 15] : 0), y = sum_upto_16(there ? wave_sum[1][lane & 15] : 0), z = sum_upto_16(there ? wave_sum[2][lane & 15] : 0);
+        tt = __builtin_amdgcn_readlane(x, 15);
+        tp = __builtin_amdgcn_readlane(y, 15);
+        tr = __builtin_amdgcn_readlane(z, 15);
+        if (wave) {
+            const uint32_t w = __builtin_amdgcn_readfirstlane(wave) - 1;
+            it = sat_add(it, __builtin_amdgcn_readlane(x, w));
+            ip = sat_add(ip, __builtin_amdgcn_readlane(y, w));
+            ir = sat_add(ir, __builtin_amdgcn_readlane(z, w));
+        }
     }
     const uint64_t taken = a.cursor[0], given = a.cursor[1];
     const uint64_t left = given > taken ? min(given - taken, (uint64_t)a.ring_size) : 0;
     const uint32_t code = bad ? ZVDB_KV_TABLE_TOO_SHORT : tt > a.slot_cap ? ZVDB_KV_SLOTS_TOO_FEW : tp > left ? ZVDB_KV_OUT_OF_PAGES : ZVDB_KV_PLANNED;
-    const bool ok = code == ZVDB_KV_PLANNED;  // then all sums fit 32 bits: slot_cap and the ring do
-    tok[tid] = (uint32_t)(it - st);
-    pag[tid] = (uint32_t)(ip - sp);
+    const bool ok = code == ZVDB_KV_PLANNED;  // then no sum is full: slot_cap and the ring are below that
+    tok[tid] = it - st;
+    pag[tid] = ip - sp;
     run[tid] = ir - sr;
     if (tid == 0) run[nt] = tr;
     if (blockIdx.x == 0) {
-        uint32_t x = (uint32_t)(it - st);
+        uint32_t x = it - st;
         for (uint32_t i = i0; i < i1; ++i) {
             const uint32_t c = a.lengths[i], f = a.fresh[i];
             a.starts[i] = ok ? x : 0;
@@ -134,12 +157,12 @@ __global__ __launch_bounds__(1024) void k_kv_plan(const KvPlanArgs a) {
             x += f;
         }
         if (tid == 0) {
-            a.starts[a.n] = ok ? (uint32_t)tt : 0;
+            a.starts[a.n] = ok ? tt : 0;
             a.out_cursor[0] = taken + (ok ? tp : 0);
             a.out_cursor[1] = given;
             a.status[0] = code;
-            a.status[1] = (uint32_t)min(tp, (uint64_t)0x7FFFFFFF);
-            a.status[2] = (uint32_t)min(tt, (uint64_t)0x7FFFFFFF);
+            a.status[1] = tp;
+            a.status[2] = tt;
             a.status[3] = 0;
         }
     }
@@ -154,12 +177,7 @@ __global__ __launch_bounds__(1024) void k_kv_plan(const KvPlanArgs a) {
         const bool mine = l16 < per && i < a.n;
         const uint32_t len = mine ? a.lengths[i] : 0, add = mine ? a.fresh[i] : 0;
         const uint32_t want = (len + add + mask) >> a.page_shift, news = want - ((len + mask) >> a.page_shift), runs = add ? want - (len >> a.page_shift) : 0;
-        uint32_t xt = add, xp = news, xr = runs;  // inclusive, over the thread's requests
-#pragma unroll
-        for (int d = 1; d < 16; d <<= 1) {
-            const uint32_t t = __shfl_up(xt, d, 16), p = __shfl_up(xp, d, 16), r = __shfl_up(xr, d, 16);
-            if (l16 >= (uint32_t)d) { xt += t; xp += p; xr += r; }
-        }
+        const uint32_t xt = sum_upto_16(add), xp = sum_upto_16(news), xr = sum_upto_16(runs);  // over the thread's requests
         const uint32_t r = (uint32_t)x - run[c];
         const uint64_t hit = __ballot(r >= xr - runs && r < xr) >> group & 0xFFFF;  // one lane's request holds the run
         const int src = __ffsll((unsigned long long)hit) - 1;
