@@ -613,7 +613,7 @@ __global__ __launch_bounds__(64 * WAVES, NB == 8 && TERMS == 3 ? 1 : NB == 8 || 
 }
 
 // Row tiles of a wave of k_kv_attend_wide: what 256 registers hold
-constexpr int wide_tiles(int nb, int terms) { return terms == 1 && nb <= 4 ? 3 : 1; }
+constexpr int wide_tiles(int nb, int terms) { return nb == 8 ? 1 : terms == 1 ? 3 : 2; }
 
 // Many rows (prompts): each of a block's four waves has NT tiles of its own and all walk the same tokens.  A wave's tile of 16 tokens (at
 // width 256 its keys or its values) is widened once for the block into LDS, in the order in which the matrix instructions take it: 64
@@ -903,11 +903,16 @@ __global__ __launch_bounds__(256, NB == 8 && TERMS == 3 ? 1 : NB == 8 || TERMS =
 // ---- launches -----------------------------------------------------------------------------------------------------------
 
 // How a call is cut.  Rows of one (request, head) that fit 64 are few: blocks of 16 whose waves divide the tokens; more of them give
-// each wave its own tiles.  Tokens are split until the card has four blocks for each unit: requests differ in length, so a good third of
-// the splits is empty.  Each part costs its start (some 5 us of dependent reads) and its place in the join: parts of few rows hold at
-// least 1,024 tokens (48 requests to 8,192 tokens: 2 / 3 / 5 splits 58.5 / 54.4 / 59.8 us; one of 32,768: 32 / 256 splits 15.5 / 28.9), and
-// two blocks a unit are left whole (64 requests of 2,048: 29.8 us, 39.8 with two splits).  Where even that leaves units empty a block
-// has eight waves (one request of 1,024 tokens: 9.6 us, 12.8 with four waves and splits).
+// each wave its own tiles, several where that makes two blocks for each unit of the card, else one (82 new tokens of 7 heads over 2,452:
+// 21.4 -> 14.6 us).
+//
+// Tokens are split where blocks are fewer than the card wants.  Each part costs its start (some 5 us of dependent reads), its rows in the
+// workspace and its place in the join, so parts have at least 1,024 tokens of few rows, 256 of many.  Few rows: four blocks for each unit
+// unless there are two (requests differ in length, a good third of the splits is empty: 48 requests to 8,192 tokens: 2 / 3 / 5 splits
+// 58.5 / 54.4 / 59.8 us; one of 32,768: 32 / 256 splits 15.5 / 28.9; 64 of 2,048: whole 29.8, two splits 39.8).  Many: none from one block
+// a unit on (7 prompts of 1,294 tokens, 294 blocks: 38 us, with four splits 82), else to two, four at width 256, whose blocks are the
+// slowest (33 rows of 8 heads over 4,100 tokens: 52 us, 70 with two).  Few rows that leave units empty even so get eight waves to a
+// block (one request of 1,024 tokens: 9.0 us, 12.8 with four waves and splits).
 struct KvCut {
     bool wide;
     uint32_t nt, tiles, splits, split_tokens, waves;
@@ -920,11 +925,18 @@ static KvCut kv_cut(const KvGeom &g, uint32_t type, uint32_t group, uint32_t n, 
     const uint32_t w = kv_width(g.dim);
     c.wide = rows > 64;
     c.nt = c.wide ? wide_tiles(w / 32, type == ZVDB_KV_F32 ? 3 : 1) : 1;
-    const uint32_t block_rows = c.wide ? 64 * c.nt : 16;
-    c.tiles = (uint32_t)((rows + block_rows - 1) / block_rows);
-    const uint64_t base = (uint64_t)g.heads * n * c.tiles;
-    const uint64_t want = (uint64_t)cus * 4;
-    uint64_t splits = base && (c.wide || base < 2 * (uint64_t)cus) ? (want + base - 1) / base : 1;
+    auto cut_rows = [&]() {
+        const uint32_t block_rows = c.wide ? 64 * c.nt : 16;
+        c.tiles = (uint32_t)((rows + block_rows - 1) / block_rows);
+        return (uint64_t)g.heads * n * c.tiles;
+    };
+    uint64_t base = cut_rows();
+    if (c.nt > 1 && base < 2 * (uint64_t)cus) {
+        c.nt = 1;
+        base = cut_rows();
+    }
+    const uint64_t want = (uint64_t)cus * (c.wide && w < 256 ? 2 : 4);
+    uint64_t splits = base && base < (c.wide ? 1 : 2) * (uint64_t)cus ? (want + base - 1) / base : 1;
     const uint32_t least = c.wide ? 256 : 1024;
     splits = std::min<uint64_t>(splits, ((uint64_t)max_length + least - 1) / least);
     splits = std::max<uint64_t>(std::min<uint64_t>(splits, 256), 1);
@@ -938,7 +950,8 @@ static KvCut kv_cut(const KvGeom &g, uint32_t type, uint32_t group, uint32_t n, 
 template <int NB, int TERMS>
 static void launch_attend_as(const KvAttendArgs &a, const KvCut &c, hipStream_t s) {
     const dim3 grid((uint32_t)c.blocks), block(64 * c.waves);
-    if (c.wide) hipLaunchKernelGGL((k_kv_attend_wide<NB, wide_tiles(NB, TERMS), TERMS>), grid, block, 0, s, a);
+    if (c.wide && c.nt > 1) hipLaunchKernelGGL((k_kv_attend_wide<NB, wide_tiles(NB, TERMS), TERMS>), grid, block, 0, s, a);
+    else if (c.wide) hipLaunchKernelGGL((k_kv_attend_wide<NB, 1, TERMS>), grid, block, 0, s, a);
     else if (c.waves == 8) hipLaunchKernelGGL((k_kv_attend<NB < 8 ? NB : 4, TERMS, 8>), grid, block, 0, s, a);
     else hipLaunchKernelGGL((k_kv_attend<NB, TERMS, 4>), grid, block, 0, s, a);
 }
