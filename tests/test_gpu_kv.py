@@ -558,3 +558,193 @@ def test_selecting_every_row_is_attending_to_all(torch):
         for h in range(8):
             _, _, bo, bl = ref.attend_row(qx[i, h], mem.k[mem.rows_of(i)][:, h // 4], mem.v[mem.rows_of(i)][:, h // 4], float(np.float32(0.1)), "fp32")
             assert (np.abs(got[i, h] - want[i, h]) <= 2 * bo).all() and abs(lse[i, h] - wl[i, h]) <= 2 * bl
+
+
+# ---- the calls together -----------------------------------------------------------------------------------------------------------
+
+class Server:
+    """A decode loop as a program runs it: plan, append, attend on a stream; lengths, cursor and tables stay on the device."""
+
+    def __init__(self, torch, n, d, heads, group, page, slot_cap, max_length, kind="bf16"):
+        import zvdb_amd as zv
+        self.torch, self.n, self.d, self.heads, self.group, self.kind, self.cap, self.max_length = torch, n, d, heads, group, kind, slot_cap, max_length
+        self.stride = -(-max_length // page)
+        pages = n * self.stride
+        self.lay = zv.KVLayout(head_dim=d, kv_heads=heads, page_size=page, pages=pages)
+        dev = dict(device="cuda")
+        i32 = dict(dtype=torch.int32, **dev)
+        self.cache = torch.full((pages * self.lay.page_bytes,), 255, dtype=torch.uint8, **dev)
+        self.ring = torch.randperm(pages, generator=torch.Generator().manual_seed(1)).to(torch.int32).cuda()
+        self.cursor, self.next_cursor = torch.tensor([0, pages], dtype=torch.int64, **dev), torch.zeros(2, dtype=torch.int64, **dev)
+        self.lengths, self.next_lengths, self.new = torch.zeros(n, **i32), torch.zeros(n, **i32), torch.zeros(n, **i32)
+        self.tables = torch.full((n, self.stride), -1, **i32)
+        self.starts, self.status = torch.zeros(n + 1, **i32), torch.zeros(4, **i32)
+        self.slots = torch.zeros(slot_cap, dtype=torch.int64, **dev)
+        dt = torch.bfloat16 if kind == "bf16" else torch.float32
+        self.qkv = torch.zeros(slot_cap, (heads * group + 2 * heads) * d, dtype=dt, **dev)  # one projection's rows: q, k, v side by side
+        self.out = torch.zeros(slot_cap, heads * group, d, dtype=dt, **dev)
+        self.lse = torch.zeros(slot_cap, heads * group, **dev)
+        self.ws = torch.empty(max(16, self.lay.attend_workspace(kv_type(kind), heads * group, n, slot_cap, slot_cap, max_length)), dtype=torch.uint8, **dev)
+
+    def step(self):
+        s, lay, row, size = stream(self.torch), self.lay, self.qkv.shape[1], self.qkv.element_size()
+        q, k = self.qkv.data_ptr(), self.qkv.data_ptr() + self.heads * self.group * self.d * size
+        v = k + self.heads * self.d * size
+        lay.plan_dev(self.lengths.data_ptr(), self.new.data_ptr(), self.n, self.ring.data_ptr(), self.ring.numel(), self.cursor.data_ptr(), self.tables.data_ptr(),
+                     self.stride, self.starts.data_ptr(), self.slots.data_ptr(), self.cap, self.next_lengths.data_ptr(), self.next_cursor.data_ptr(),
+                     self.status.data_ptr(), s)
+        lay.append_dev(self.cache.data_ptr(), k, row, v, row, kv_type(self.kind), self.cap, self.slots.data_ptr(), s)
+        lay.attend_dev(self.cache.data_ptr(), q, row, kv_type(self.kind), self.heads * self.group, self.n, self.starts.data_ptr(), self.cap, self.cap,
+                       self.next_lengths.data_ptr(), self.tables.data_ptr(), self.stride, self.max_length, 0.17, True, self.ws.data_ptr(), self.ws.numel(),
+                       self.out.data_ptr(), self.lse.data_ptr(), s)
+        self.lengths.copy_(self.next_lengths)
+        self.cursor.copy_(self.next_cursor)
+
+
+def serve_and_check(torch, server, rounds, run, rng):
+    """rounds: new tokens of each request, step by step; every row of every step against the restatement."""
+    n, d, heads, group = server.n, server.d, server.heads, server.group
+    keys, vals = [np.zeros((0, heads, d)) for _ in range(n)], [np.zeros((0, heads, d)) for _ in range(n)]
+    scale = float(np.float32(0.17))
+    for new in rounds:
+        total = sum(new)
+        x, xx = as_type(torch, rng.standard_normal((server.cap, server.qkv.shape[1])) * 1.3, server.kind)
+        server.qkv.copy_(x)
+        server.new.copy_(torch.tensor(new, dtype=torch.int32))
+        run()
+        torch.cuda.synchronize()
+        assert server.status.tolist()[0] == 0 and server.starts.tolist()[-1] == total
+        got, lse = server.out.double().cpu().numpy(), server.lse.double().cpu().numpy()
+        at = 0
+        for i, m in enumerate(new):
+            part = xx[at:at + m]
+            qw, kw = heads * group * d, heads * d
+            for store, rows in ((keys, part[:, qw:qw + kw]), (vals, part[:, qw + kw:])):
+                rows = rows.reshape(m, heads, d)
+                store[i] = np.concatenate([store[i], np.stack([ref.encode_rows(rows[:, h], d)[2] for h in range(heads)], 1)]) if m else store[i]
+            for j in range(m):
+                see = len(keys[i]) - m + j + 1
+                for h in range(heads * group):
+                    o, l, bo, bl = ref.attend_row(part[j, h * d:(h + 1) * d], keys[i][:see, h // group], vals[i][:see, h // group], scale, server.kind)
+                    assert (np.abs(got[at + j, h] - o) <= bo).all() and abs(lse[at + j, h] - l) <= bl, (i, j, h)
+            at += m
+    return [len(k) for k in keys]
+
+
+ROUNDS = [[5, 0, 17, 1], [1, 1, 1, 1], [1, 0, 1, 1], [3, 2, 0, 30], [1, 1, 1, 1], [0, 0, 0, 0], [16, 1, 1, 7], [1, 1, 1, 1]]
+
+
+@pytest.mark.parametrize("kind", ["bf16", "fp32"])
+@pytest.mark.parametrize("d,heads,group,page", [(64, 2, 2, 16), (128, 1, 3, 32)])
+def test_serving_step_by_step(torch, kind, d, heads, group, page):
+    server = Server(torch, 4, d, heads, group, page, 36, 128, kind)
+    lengths = serve_and_check(torch, server, ROUNDS, server.step, np.random.default_rng(31))
+    assert server.lengths.tolist() == lengths
+
+
+def test_serving_on_another_stream(torch):
+    server = Server(torch, 4, 64, 2, 2, 16, 36, 128)
+    other = torch.cuda.Stream()
+
+    def run():
+        other.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(other):
+            server.step()
+        torch.cuda.current_stream().wait_stream(other)
+    serve_and_check(torch, server, ROUNDS, run, np.random.default_rng(32))
+
+
+@pytest.mark.parametrize("max_length", [128, 4096])  # the second is split: workspace and join in the graph
+def test_serving_from_a_graph(torch, max_length):
+    """The step captured once and replayed for every round, whatever the lengths are; other work of the program in between."""
+    server = Server(torch, 4, 64, 2, 2, 16, 36, max_length)
+    warm = torch.cuda.Stream()
+    with torch.cuda.stream(warm):
+        server.step()  # no new tokens: nothing changes
+    warm.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        server.step()
+    noise = torch.randn(512, 512, device="cuda")
+
+    def run():
+        graph.replay()
+        torch.cuda.synchronize()
+        (noise @ noise).sum().item()
+    serve_and_check(torch, server, ROUNDS, run, np.random.default_rng(33))
+
+
+def test_two_servers_on_two_streams(torch):
+    """Two caches with workspaces of their own, their steps in flight together."""
+    servers, streams = [Server(torch, 4, 64, 1, 4, 16, 36, 2048) for _ in range(2)], [torch.cuda.Stream() for _ in range(2)]
+    alone = [Server(torch, 4, 64, 1, 4, 16, 36, 2048) for _ in range(2)]
+    rng = np.random.default_rng(34)
+    for new in ROUNDS:
+        for x, y in zip(servers, alone):
+            x.qkv.copy_(as_type(torch, rng.standard_normal(tuple(x.qkv.shape)), "bf16")[0])
+            y.qkv.copy_(x.qkv)
+            for z in (x, y):
+                z.new.copy_(torch.tensor(new, dtype=torch.int32))
+        torch.cuda.synchronize()
+        for x, s in zip(servers, streams):
+            with torch.cuda.stream(s):
+                x.step()
+        torch.cuda.synchronize()
+        for x, y in zip(servers, alone):
+            y.step()
+            torch.cuda.synchronize()
+            total = sum(new)
+            assert torch.equal(x.out[:total], y.out[:total]) and torch.equal(x.lse[:total], y.lse[:total]) and torch.equal(x.cache, y.cache)
+
+
+def test_a_full_ring_stops_the_step_and_nothing_else(torch):
+    server = Server(torch, 2, 64, 1, 1, 16, 40, 64)
+    server.new.copy_(torch.tensor([20, 20], dtype=torch.int32))
+    server.step()                            # two pages each
+    server.cursor[1] = server.cursor[0] + 1  # one left
+    server.new.copy_(torch.tensor([20, 20], dtype=torch.int32))  # 40 tokens: a page more for each
+    before = [t.clone() for t in (server.cache, server.tables, server.lengths, server.cursor)]
+    server.out.fill_(9.0)
+    server.step()
+    torch.cuda.synchronize()
+    assert server.status.tolist() == [1, 2, 40, 0]
+    assert all(torch.equal(a, b) for a, b in zip(before, (server.cache, server.tables, server.lengths, server.cursor))) and (server.out == 9.0).all()
+    server.new.copy_(torch.tensor([20, 0], dtype=torch.int32))   # the one that is left is enough for one of them
+    server.step()
+    torch.cuda.synchronize()
+    assert server.status.tolist() == [0, 1, 20, 0] and server.lengths.tolist() == [40, 20] and (server.out[:20] != 9.0).any() and (server.out[20:] == 9.0).all()
+
+
+@pytest.mark.parametrize("mode", ["f32", "bf16"])
+def test_searching_an_index_and_attending_to_what_it_found(torch, mode):
+    """Keys of each head in an index of the framework (dot product), its search's ids and counts straight into the attention over the
+    same tokens' keys and values in 4 bits."""
+    import zvdb_amd as zv
+    rng = np.random.default_rng(41)
+    tokens, d, heads, n, k = 900, 64, 2, 5, 12
+    mem = Memory(torch, rng, [tokens], d, heads, 16)
+    mem.lengths, mem.tables = [tokens] * n, np.repeat(mem.tables, n, 0)   # one memory that every request reads
+    q, qx = as_type(torch, rng.standard_normal((n, heads, d)), "fp32")
+    ids = torch.zeros((heads, n, k), dtype=torch.int64, device="cuda")
+    dist = torch.zeros((heads, n, k), dtype=torch.float32, device="cuda")
+    counts = torch.zeros((heads, n), dtype=torch.int32, device="cuda")
+    m, s, keep = zv.BF_F32 if mode == "f32" else zv.BF_BF16, stream(torch), []
+    for h in range(heads):
+        idx = zv.Index(dim=d, metric=zv.METRIC_DOT, capacity=tokens, flags=zv.FLAG_BF16_MIRROR)
+        idx.add(mem.k[:, h].astype(np.float32))
+        wsb = idx.bruteforce_workspace(n, k, m)
+        ws, qh = torch.empty(wsb, dtype=torch.uint8, device="cuda"), q[:, h].contiguous()
+        idx.search_bruteforce_dev(qh.data_ptr(), n, d, k, m, 0, ws.data_ptr(), wsb, ids[h].data_ptr(), dist[h].data_ptr(), counts[h].data_ptr(), s)
+        keep += [idx, ws, qh]
+    out, lse = torch.zeros_like(q), torch.zeros((n, heads), device="cuda")
+    L, T = mem.i32(mem.lengths), mem.i32(mem.tables)
+    mem.lay.attend_selected_dev(mem.cache.data_ptr(), q.data_ptr(), heads * d, zv.KV_F32, heads, n, ids.data_ptr(), counts.data_ptr(), k, L.data_ptr(), T.data_ptr(),
+                                mem.stride, 0.125, out.data_ptr(), lse.data_ptr(), s)
+    torch.cuda.synchronize()
+    got, gl = out.double().cpu().numpy(), lse.double().cpu().numpy()
+    for i in range(n):
+        for h in range(heads):
+            best = np.argsort(-(mem.k[:, h] @ qx[i, h]), kind="stable")[:k]
+            assert set(best.tolist()) == set(ids[h, i].tolist()) and counts[h, i] == k
+            o, l, bo, bl = ref.attend_row(qx[i, h], mem.k[best, h], mem.v[best, h], 0.125, "fp32")
+            assert (np.abs(got[i, h] - o) <= bo).all() and abs(gl[i, h] - l) <= bl
