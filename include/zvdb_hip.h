@@ -434,7 +434,8 @@ int zvdb_hip_timing_read(zvdb_hip_index *h, double *out_total_ms, uint32_t *out_
  * them -- over whole requests, or over the rows whose ids a search of this library returned.  The calls hold no state: the
  * cache, its block tables and every length are the caller's device memory, every call is a _dev call (device pointers, the
  * caller's stream, nothing allocated, nothing synchronised: a captured call replays).  All pointers of a call are memory of
- * ONE device, which need not be the current one, and so is the stream's; arrays of rows are 16-byte aligned.
+ * ONE device, which need not be the current one, and so is the stream's; arrays of rows are 16-byte aligned; what a call writes
+ * overlaps nothing that it reads.
  *
  * Cache: `pages` pages of zvdb_hip_kv_page_bytes each, one after the other.  A page holds page_size tokens of every head; of
  * each head, with D = head_dim padded to 64, 128 or 256 (padding holds zeros) and NB = D / 32:
@@ -490,7 +491,7 @@ int zvdb_hip_kv_append_dev(const zvdb_hip_kv_layout *layout, void *d_cache, cons
 /* Reads rows back, widened exactly: d_k, d_v [n][kv_heads][head_dim] of `type` (either may be NULL); zeros where there is no slot. */
 int zvdb_hip_kv_read_dev(const zvdb_hip_kv_layout *layout, const void *d_cache, const void *d_slots, uint32_t n, void *d_k, void *d_v, uint32_t type, void *stream);
 
-/* Attention of new tokens over their requests, o = softmax(scale q K^T) V with fp32 sums.  d_q: [rows][q_heads][head_dim] of `type`,
+/* Attention of new tokens over their requests, o = softmax(scale q K^T) V with fp32 sums; 0 < scale <= 1e38.  d_q: [rows][q_heads][head_dim] of `type`,
  * q_stride elements from one token to the next (a multiple of 8); request i has the rows d_starts[i] .. d_starts[i + 1] (at most
  * max_new of them; d_starts as zvdb_hip_kv_plan_dev writes it) and d_lengths[i] tokens (at most max_length), its new ones included.
  * Query head h reads key/value head h / (q_heads / kv_heads).  causal: the j-th of m new tokens sees the tokens before position

@@ -547,6 +547,15 @@ def test_selected_rows_of_hidden_pages_and_nan(torch):
     check_selected(mem, got, lse, qx, ids, None, 2, "bf16", float(np.float32(0.3)), there=lambda i, t: not (i == 0 and t // 16 == 4))
 
 
+def test_lists_of_no_rows(torch):
+    rng = np.random.default_rng(23)
+    mem = Memory(torch, rng, [40, 0], 64, 2, 16)
+    q, _ = as_type(torch, rng.standard_normal((2, 4, 64)), "bf16")
+    for ids, counts in ((np.zeros((2, 2, 0), np.uint64), None), (np.full((2, 2, 5), 2**64 - 1, np.uint64), None), (np.zeros((2, 2, 5), np.uint64), np.zeros((2, 2)))):
+        got, lse = selected(mem, q, ids, counts, 2, "bf16", 0.3)
+        assert (got[:2] == 0).all() and np.isneginf(lse[:2]).all()
+
+
 def test_selecting_every_row_is_attending_to_all(torch):
     rng = np.random.default_rng(22)
     mem = Memory(torch, rng, [130, 64], 128, 2, 16)

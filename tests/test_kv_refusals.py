@@ -64,7 +64,7 @@ def attend(lay, cache=A, q=A, q_stride=256, type=1, heads=4, n=2, starts=A, rows
 @pytest.mark.parametrize("bad", [dict(cache=0), dict(q=0), dict(starts=0), dict(lengths=0), dict(tables=0), dict(out=0), dict(q=A + 8), dict(out=A + 8),
                                  dict(cache=A + 8), dict(type=2), dict(heads=1), dict(heads=3), dict(heads=0), dict(q_stride=248), dict(q_stride=260),
                                  dict(stride=0), dict(scale=0.0), dict(scale=-1.0), dict(scale=float("nan")), dict(scale=float("inf")), dict(n=1 << 24),
-                                 dict(rows=2**31), dict(max_length=2**31)])
+                                 dict(rows=2**31), dict(max_length=2**31), dict(scale=3e38), dict(rows=2**30, max_new=2**30, heads=4)])
 def test_attend_refuses(bad):
     refused(lambda: attend(layout(), **bad))
 

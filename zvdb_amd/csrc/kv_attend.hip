@@ -12,8 +12,9 @@
 // four tokens of V, a 4-byte load their four scales.  v_cvt_scalef32_pk_bf16_fp4 applies the block's scale while it widens: a code
 // times a power of two is a bf16 number, so K and V lose nothing on the way into the matrix instructions.
 //
-// Rounding.  bf16 queries: products and sums are fp32; P is rounded to bf16 (2^-9 relative, signs at random, below the rounding of
-// the bf16 output), the sum of P is of the unrounded values.  fp32 queries: q and P are split into three bf16 terms each (24 bits,
+// Rounding.  bf16 queries: products and sums are fp32; P is rounded to bf16 for its product with V (at most 2^-8 of each weight, as the
+// output's own rounding, and at random: 2.1e-3 off the 64-bit result in norm where rounding the exact result alone is 1.7e-3), the sum of
+// P is of the unrounded values.  fp32 queries: q and P are split into three bf16 terms each (24 bits,
 // exact for q) and every product runs three times.
 //
 // The maximum is lazy: m moves only when a score exceeds it by more than 2^kSlack (a wave-wide vote, no exchange between lanes);
@@ -32,7 +33,7 @@ struct KvAttendArgs {
     void *out;
     float *lse;
     const uint32_t *starts, *lengths, *tables;
-    float *part;  // [rows][q heads][splits][dim + 2]: O (not divided), m, l
+    float *part;  // [rows][q heads][splits][dim + 4]: O (not divided), m, l
     const uint64_t *ids;
     const uint32_t *counts;
     uint64_t q_stride;
@@ -523,7 +524,10 @@ __device__ inline void store_rows(const KvAttendArgs &a, const KvBlock &blk, con
 }
 
 // Few rows (decode): 16 of them to a block, whose waves take the chunks of the split's tokens in turn and are joined in LDS.  Each wave
-// widens what it loads, one chunk of 32 tokens ahead.
+// widens what it loads, one chunk of 32 tokens ahead: 4.3 KB at width 128, three waves on a SIMD.  Bound by HBM: 48 requests to 8,192
+// tokens, 8 x 128, bf16: 223 MB in 54 us with the join, 53 with the loads alone and no arithmetic; with fp32 queries, whose products run
+// three times, by the instructions around them (3 requests to 131,072 tokens, 4 x 64: 88 MB in 35 us, 30 with the loads alone).  One
+// masked step serves whole and cut chunks: two copies of it took 232 registers for 128 and one wave less.
 template <int NB, int TERMS, int WAVES>
 __global__ __launch_bounds__(64 * WAVES, NB == 8 && TERMS == 3 ? 1 : NB == 8 || TERMS == 3 || WAVES == 8 ? 2 : NB == 4 ? 3 : 4) void k_kv_attend(const KvAttendArgs a) {
     constexpr uint32_t STRIDE = 32 * WAVES;
@@ -619,6 +623,13 @@ constexpr int wide_tiles(int nb, int terms) { return nb == 8 ? 1 : terms == 1 ? 
 // width 256 its keys or its values) is widened once for the block into LDS, in the order in which the matrix instructions take it: 64
 // tokens (32) at a time into one of two buffers while the other is read, one barrier for each.  A wave's next raw rows are requested as
 // soon as it has widened the last, a whole chunk ahead.
+//
+// Bound by instruction issue: 32 tokens x 48 rows are 48 matrix instructions (768 cycles of the unit) and some 190 others, of which the
+// weights are two thirds; two waves on a SIMD overlap them in part.  4 prompts of 1,500 to 2,048 tokens, 32 heads, causal: 275 us, 0.90
+// PFLOP/s, where a library product of 8192^3 reaches 1.21.  Taken and measured: every wave widening for itself 331 us; 32 or 64 rows a
+// wave 297 / 666 (registers); three waves of 32 rows on a SIMD 291; eight waves sharing a widened tile 300; raised priority around the
+// matrix instructions 308.  At width 256 a wave has 16 rows and the start and end of a block weigh as much as its 20 chunks (33 rows of 8
+// heads over 4,100 tokens: 51 us; two tiles a wave at one wave a SIMD 78; keys widened by every wave 86).
 template <int NB, int NT, int TERMS>
 __global__ __launch_bounds__(256, NB == 8 && TERMS == 3 ? 1 : 2) void k_kv_attend_wide(const KvAttendArgs a) {
     constexpr uint32_t TILES = NB == 8 ? 2 : 4, T = 16 * TILES;
@@ -804,7 +815,8 @@ __global__ __launch_bounds__(256) void k_kv_join(const KvAttendArgs a) {
 // A block takes one request and key/value head: its list of ids is resolved to places in the cache in LDS (a search's ids and counts
 // as zvdb_hip_search_*_dev writes them), then its four waves take 32 entries at a time.  A list of 100 is three dependent reads (ids,
 // pages, rows) and one chunk to a wave, so what counts is how many blocks a unit holds; a token's V lies in 16 pieces of four tokens
-// each, of which the other three are read for nothing.
+// each, of which the other three are read for nothing.  256 requests x 8 heads x 100 rows of 65,536, 4 x 128: 16.5 us; the 128-byte lines
+// that it touches are 131 MB (640 bytes for a row's 136), 7.9 TB/s of them out of the caches.
 constexpr uint32_t kSelPass = 1024;  // entries resolved at a time
 
 template <int NB, int TERMS>
@@ -978,7 +990,7 @@ static int check_queries(const KvGeom &g, const void *q, uint64_t q_stride, uint
     KV_ARG(q && out && cache, "null argument");
     KV_ARG(kv_aligned(q, 16) && kv_aligned(out, 16) && kv_aligned(cache, 16), "kv_attend: cache, q and out need 16-byte alignment");
     KV_ARG(q_stride >= (uint64_t)q_heads * g.dim && q_stride % 8 == 0, "kv_attend: a token's stride is at least q_heads * head_dim and a multiple of 8");
-    KV_ARG(scale > 0.0f && scale <= FLT_MAX, "kv_attend: scale %g (positive and finite)", (double)scale);
+    KV_ARG(scale > 0.0f && scale <= 1e38f, "kv_attend: scale %g (positive, at most 1e38)", (double)scale);
     (void)type;
     return ZVDB_OK;
 }
@@ -992,6 +1004,8 @@ static int check_heads(const KvGeom &g, uint32_t type, uint32_t q_heads) {
 static int attend_shape(const KvGeom &g, uint32_t type, uint32_t q_heads, uint32_t n, uint32_t rows, uint32_t max_new, uint32_t max_length) {
     ZV_CHECK(check_heads(g, type, q_heads));
     KV_ARG(n < (1u << 24) && rows < 0x7FFFFFFFu && max_new < 0x7FFFFFFFu && max_length < 0x7FFFFFFFu, "kv_attend: a size is out of range");
+    KV_ARG((uint64_t)std::min(max_new, rows) * (q_heads / g.heads) < 0x7FFFFFFFu, "kv_attend: %u rows of %u heads each are too many for one request", std::min(max_new, rows),
+           q_heads / g.heads);
     return ZVDB_OK;
 }
 
