@@ -308,6 +308,28 @@ def test_long_contexts_are_split_and_joined(torch, kind, d, heads, group, page):
 
 
 @pytest.mark.parametrize("kind", ["bf16", "fp32"])
+@pytest.mark.parametrize("d,heads,group,page", [(64, 1, 2, 16), (40, 2, 1, 32), (128, 1, 3, 16), (104, 1, 2, 64), (256, 1, 2, 64), (248, 1, 1, 128)])
+@pytest.mark.parametrize("bound,splits", [(2500, 3), (8192, 8), (9216, 9), (262_144, None)])
+def test_every_number_of_splits(torch, kind, d, heads, group, page, bound, splits):
+    # the host's bound says how many splits there are; the requests fill some of them, and a NaN key and a NaN value are in one each
+    lengths, new = [2400, 0, 1, 2100, 1025], [1, 1, 1, 1, 1]
+
+    def spoil(mem, k, v):
+        k[mem.first[3] + 2099, 0, 1] = np.nan
+        v[mem.first[4] + 1024, 0, d - 1] = np.inf
+
+    with np.errstate(invalid="ignore"):
+        *_, size = check_attend(torch, lengths, new, d, heads, group, page, kind, True, spoil=spoil, max_length=bound)
+    part = len(new) * heads * group * (d + 4) * 4
+    assert size == part * splits if splits else size > 9 * part
+
+
+def test_the_largest_number_of_splits(torch):
+    *_, size = check_attend(torch, [2100], [1], 64, 1, 2, 16, "bf16", True, max_length=262_144)
+    assert size == 2 * 256 * (64 + 4) * 4
+
+
+@pytest.mark.parametrize("kind", ["bf16", "fp32"])
 @pytest.mark.parametrize("causal", [True, False])
 @pytest.mark.parametrize("d,heads,group,page", [(64, 2, 2, 16), (128, 1, 4, 32), (72, 1, 5, 16), (256, 1, 2, 64)])
 def test_prompts(torch, kind, causal, d, heads, group, page):
