@@ -157,7 +157,8 @@ def special_rows(rng, n, heads, d):
 
 @pytest.mark.parametrize("d,heads,page,n,kind", [(64, 1, 16, 1, "bf16"), (64, 3, 16, 37, "fp32"), (8, 2, 32, 21, "fp32"), (72, 2, 64, 33, "bf16"), (96, 4, 16, 50, "fp32"),
                                                  (128, 8, 128, 29, "bf16"), (128, 1, 16, 100, "fp32"), (136, 3, 16, 17, "bf16"), (256, 2, 256, 65, "bf16"),
-                                                 (256, 1, 32, 40, "fp32")])
+                                                 (256, 1, 32, 40, "fp32"), (64, 5, 16, 70, "bf16"), (48, 7, 16, 19, "fp32"), (120, 5, 64, 31, "bf16"), (128, 6, 16, 40, "fp32"),
+                                                 (128, 9, 32, 18, "bf16"), (200, 5, 16, 23, "bf16"), (256, 7, 64, 11, "fp32")])
 def test_append_and_read_bit_for_bit(torch, d, heads, page, n, kind):
     import zvdb_amd as zv
     rng = np.random.default_rng(d + n)

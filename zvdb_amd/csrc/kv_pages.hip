@@ -223,62 +223,72 @@ __device__ inline void kv_load8(const T *p, float *x) {
 // magnitude over E2M1's 4 -- the next one from 7/4 of it on, where 6 would be nearer than 8 and the largest element would lose an
 // eighth and more of itself.  A power of two divides exactly, so the code is the nearest of x / scale, ties to even (bf16 rows
 // meet ties often: 8 significant bits over a grid of 3), saturating at 6.  Lanes of one wave hold consecutive tokens of ONE head:
-// the four tokens of a V group are written by neighbouring lanes into the same 16 pieces, and the blocks of one token's heads stand side
-// by side.  Bound by HBM: 32,771 rows of 8 x 96 fp32, keys and values: 272 MB in 47 us, 5.8 TB/s.
+// the four tokens of a V group are written by neighbouring lanes into the same 16 pieces.  A lane takes two heads of its token, so that
+// more of what it reads is in flight and in one place (65,537 rows of 8 x 128 bf16, keys and values, buffers in turn: one head a lane 89 us,
+// two 72, four 71, eight 76; 40,000 of 5 x 64 fp32: 23.4, 23.4, 27.3, 25.1).  Bound by HBM: 340 MB in 72 us, 4.7 TB/s; 32,771 rows of 8 x 96
+// fp32: 237 MB in 46 us, 5.2 TB/s.  Loads that pass the caches by: 70.7 and 48.4 us, 8,192 rows 11.2 for 9.9; not taken.
+constexpr int kAppendHeads = 2;
+
 template <class T, int NB>
 __global__ __launch_bounds__(256) void k_kv_append(uint8_t *cache, const KvGeom g, const T *k, uint64_t k_stride, const T *v, uint64_t v_stride,
                                                    const uint64_t *slots, uint32_t n) {
     constexpr uint32_t L = 4 * NB;  // lanes of a row
-    const uint32_t c8 = threadIdx.x % L, head = blockIdx.x % g.heads;
-    const uint64_t i = (uint64_t)(blockIdx.x / g.heads) * (256 / L) + threadIdx.x / L;
+    const uint32_t c8 = threadIdx.x % L, groups = (g.heads + kAppendHeads - 1) / kAppendHeads, head0 = blockIdx.x % groups * kAppendHeads;
+    const uint64_t i = (uint64_t)(blockIdx.x / groups) * (256 / L) + threadIdx.x / L;
     if (i >= n) return;  // (whole rows leave: the four lanes of a block stay together)
     const uint64_t slot = slots[i];
     if (slot >= (uint64_t)g.pages << g.page_shift) return;
     const bool value = blockIdx.y;
-    const T *src = (value ? v + i * v_stride : k + i * k_stride) + (uint64_t)head * g.dim + c8 * 8;
-    float x[8] = {};
-    if (c8 * 8 < g.dim) kv_load8(src, x);
-    uint32_t top = 0;
+    const T *src = (value ? v + i * v_stride : k + i * k_stride) + (uint64_t)head0 * g.dim + c8 * 8;
+    float x[kAppendHeads][8] = {};
 #pragma unroll
-    for (int j = 0; j < 8; ++j) top = max(top, __float_as_uint(x[j]) & 0x7FFFFFFFu);
-    top = max(top, (uint32_t)__shfl_xor((int)top, 1));
-    top = max(top, (uint32_t)__shfl_xor((int)top, 2));
-    const int e = (int)((top + 0x200000u) >> 23) - 2;
-    uint32_t b = (uint32_t)min(max(e, (int)kKvScaleMin), (int)kKvScaleMax), code = 0;
-    if (top >= 0x7F800000u) {
-        b = kKvScaleNaN;
-    } else {
-        const float s = __uint_as_float(b << 23);
-        code = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(code, x[0], x[1], s, 0);
-        code = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(code, x[2], x[3], s, 1);
-        code = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(code, x[4], x[5], s, 2);
-        code = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(code, x[6], x[7], s, 3);
-    }
+    for (int h = 0; h < kAppendHeads; ++h)
+        if (head0 + h < g.heads && c8 * 8 < g.dim) kv_load8(src + (uint64_t)h * g.dim, x[h]);
     const uint32_t t = (uint32_t)slot & (g.page_size - 1), half = g.page_size * 16 * NB;
-    uint8_t *const at = cache + (slot >> g.page_shift) * g.page_bytes + (uint64_t)head * g.head_bytes;
-    uint8_t *const scales = at + 2 * half;
-    if (!value) {
-        *reinterpret_cast<uint32_t *>(at + t * (16 * NB) + c8 * 4) = code;
-        if (c8 % 4 == 0) scales[t * NB + c8 / 4] = (uint8_t)b;
-    } else {
-        uint8_t *const w = at + half;
-        if constexpr (NB == 2) {
-            *reinterpret_cast<uint16_t *>(w + kv_v_offset<NB>(t, 2 * c8)) = (uint16_t)code;
-            *reinterpret_cast<uint16_t *>(w + kv_v_offset<NB>(t, 2 * c8 + 1)) = (uint16_t)(code >> 16);
-        } else if constexpr (NB == 4) {
-            *reinterpret_cast<uint32_t *>(w + kv_v_offset<NB>(t, c8)) = code;
+    uint8_t *at = cache + (slot >> g.page_shift) * g.page_bytes + (uint64_t)head0 * g.head_bytes;
+#pragma unroll
+    for (int h = 0; h < kAppendHeads; ++h, at += g.head_bytes) {
+        if (head0 + h >= g.heads) break;
+        uint32_t top = 0;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) top = max(top, __float_as_uint(x[h][j]) & 0x7FFFFFFFu);
+        top = max(top, (uint32_t)__shfl_xor((int)top, 1));
+        top = max(top, (uint32_t)__shfl_xor((int)top, 2));
+        const int e = (int)((top + 0x200000u) >> 23) - 2;
+        uint32_t b = (uint32_t)min(max(e, (int)kKvScaleMin), (int)kKvScaleMax), code = 0;
+        if (top >= 0x7F800000u) {
+            b = kKvScaleNaN;
         } else {
-            *reinterpret_cast<uint32_t *>(w + kv_v_offset<NB>(t, c8 / 2) + (c8 % 2) * 4) = code;
+            const float s = __uint_as_float(b << 23);
+            code = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(code, x[h][0], x[h][1], s, 0);
+            code = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(code, x[h][2], x[h][3], s, 1);
+            code = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(code, x[h][4], x[h][5], s, 2);
+            code = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(code, x[h][6], x[h][7], s, 3);
         }
-        if (c8 % 4 == 0) scales[g.page_size * NB + (t >> 2) * (4 * NB) + c8 + (t & 3)] = (uint8_t)b;
+        uint8_t *const scales = at + 2 * half;
+        if (!value) {
+            *reinterpret_cast<uint32_t *>(at + t * (16 * NB) + c8 * 4) = code;
+            if (c8 % 4 == 0) scales[t * NB + c8 / 4] = (uint8_t)b;
+        } else {
+            uint8_t *const w = at + half;
+            if constexpr (NB == 2) {
+                *reinterpret_cast<uint16_t *>(w + kv_v_offset<NB>(t, 2 * c8)) = (uint16_t)code;
+                *reinterpret_cast<uint16_t *>(w + kv_v_offset<NB>(t, 2 * c8 + 1)) = (uint16_t)(code >> 16);
+            } else if constexpr (NB == 4) {
+                *reinterpret_cast<uint32_t *>(w + kv_v_offset<NB>(t, c8)) = code;
+            } else {
+                *reinterpret_cast<uint32_t *>(w + kv_v_offset<NB>(t, c8 / 2) + (c8 % 2) * 4) = code;
+            }
+            if (c8 % 4 == 0) scales[g.page_size * NB + (t >> 2) * (4 * NB) + c8 + (t & 3)] = (uint8_t)b;
+        }
     }
 }
 
 // ---- read ---------------------------------------------------------------------------------------------------------------
 
-// Rows read back are not read again here: stores that pass the caches by (65,537 rows of 8 x 128 bf16: 93 -> 56 us)
+// Rows read back are not read again here: their stores pass the caches by (65,537 rows of 8 x 128 bf16: 51 us, 68 without).
 template <class T>
-__device__ inline void kv_store8(T *p, const float *x) {
+__device__ inline void kv_store16(T *p, const float *x) {
     if constexpr (sizeof(T) == 2) {  // a code times a power of two is a bf16 number: nothing is rounded
         uint32_t w[4];
 #pragma unroll
@@ -286,55 +296,66 @@ __device__ inline void kv_store8(T *p, const float *x) {
         __builtin_nontemporal_store(u32x4{w[0], w[1], w[2], w[3]}, reinterpret_cast<u32x4 *>(p));
     } else {
         __builtin_nontemporal_store(f32x4{x[0], x[1], x[2], x[3]}, reinterpret_cast<f32x4 *>(p));
-        __builtin_nontemporal_store(f32x4{x[4], x[5], x[6], x[7]}, reinterpret_cast<f32x4 *>(p + 4));
     }
 }
 
-// The append's lanes the other way round; a slot that is not in the cache reads as zeros.  Bound by HBM: 65,537 rows of 8 x 128 to bf16,
-// keys and values: 340 MB in 55 us, 6.2 TB/s.
+// The append the other way round; a slot that is not in the cache reads as zeros.  A lane makes 16 bytes of a row, so that every store
+// fills whole lines (8 fp32 elements to a lane, two stores of half a line each: 102 us where this takes 71, append included), and takes
+// four heads of its token: what a block writes lies together, and four loads are on their way at once (heads 1 / 2 / 4 / 8 a lane: 92 / 69 / 62 /
+// 65 us).  Bound by HBM: 65,537 rows of 8 x 128 to bf16, keys and values: 340 MB in 51 us into one pair of buffers, in 62 into four in
+// turn, 5.5 TB/s.
+constexpr int kReadHeads = 4;
+
 template <class T, int NB>
 __global__ __launch_bounds__(256) void k_kv_read(const uint8_t *cache, const KvGeom g, const uint64_t *slots, uint32_t n, T *k, T *v) {
-    constexpr uint32_t L = 4 * NB;
-    const uint32_t c8 = threadIdx.x % L, head = blockIdx.x % g.heads;
-    const uint64_t i = (uint64_t)(blockIdx.x / g.heads) * (256 / L) + threadIdx.x / L;
+    constexpr uint32_t E = 16 / sizeof(T), L = 32 * NB / E;  // elements of a lane, lanes of a row
+    const uint32_t col = threadIdx.x % L * E, groups = (g.heads + kReadHeads - 1) / kReadHeads, head0 = blockIdx.x % groups * kReadHeads;
+    const uint64_t i = (uint64_t)(blockIdx.x / groups) * (256 / L) + threadIdx.x / L;
     const bool value = k == nullptr || blockIdx.y;
     T *const dst = value ? v : k;
-    if (i >= n || c8 * 8 >= g.dim) return;
+    if (i >= n || col >= g.dim) return;
     const uint64_t slot = slots[i];
-    float x[8] = {};
+    uint32_t code[kReadHeads] = {}, b[kReadHeads] = {};
     if (slot < (uint64_t)g.pages << g.page_shift) {
         const uint32_t t = (uint32_t)slot & (g.page_size - 1), half = g.page_size * 16 * NB;
-        const uint8_t *const at = cache + (slot >> g.page_shift) * g.page_bytes + (uint64_t)head * g.head_bytes;
-        const uint8_t *const scales = at + 2 * half;
-        uint32_t code, b;
-        if (!value) {
-            code = *reinterpret_cast<const uint32_t *>(at + t * (16 * NB) + c8 * 4);
-            b = scales[t * NB + c8 / 4];
-        } else {
-            const uint8_t *const w = at + half;
-            if constexpr (NB == 2)
-                code = *reinterpret_cast<const uint16_t *>(w + kv_v_offset<NB>(t, 2 * c8)) |
-                       (uint32_t)*reinterpret_cast<const uint16_t *>(w + kv_v_offset<NB>(t, 2 * c8 + 1)) << 16;
-            else if constexpr (NB == 4)
-                code = *reinterpret_cast<const uint32_t *>(w + kv_v_offset<NB>(t, c8));
-            else
-                code = *reinterpret_cast<const uint32_t *>(w + kv_v_offset<NB>(t, c8 / 2) + (c8 % 2) * 4);
-            b = scales[g.page_size * NB + (t >> 2) * (4 * NB) + (c8 & ~3u) + (t & 3)];
-        }
-        const float s = __uint_as_float(b << 23);
-        const bf16x2 y[4] = {__builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(code, s, 0), __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(code, s, 1),
-                             __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(code, s, 2), __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(code, s, 3)};
+        const uint8_t *const first = cache + (slot >> g.page_shift) * g.page_bytes + (uint64_t)head0 * g.head_bytes;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) x[j] = b == kKvScaleNaN ? __uint_as_float(0x7FC00000u) : (float)y[j / 2][j % 2];
+        for (int h = 0; h < kReadHeads; ++h) {
+            if (head0 + h >= g.heads) break;
+            const uint8_t *const at = first + (uint64_t)h * g.head_bytes, *const scales = at + 2 * half;
+            const uint8_t *const w = value ? at + half + kv_v_offset<NB>(t, col / (2 * NB)) + col % (2 * NB) / 2 : at + t * (16 * NB) + col / 2;
+            if constexpr (E == 4) code[h] = *reinterpret_cast<const uint16_t *>(w);
+            else if constexpr (NB == 2)
+                code[h] = *reinterpret_cast<const uint16_t *>(w) |
+                          (uint32_t)*reinterpret_cast<const uint16_t *>(value ? at + half + kv_v_offset<NB>(t, col / 4 + 1) : w + 2) << 16;
+            else code[h] = *reinterpret_cast<const uint32_t *>(w);
+            b[h] = value ? scales[g.page_size * NB + (t >> 2) * (4 * NB) + (col / 32) * 4 + (t & 3)] : scales[t * NB + col / 32];
+        }
     }
-    kv_store8(dst + ((i * g.heads + head) * g.dim + c8 * 8), x);
+    T *const out = dst + (i * g.heads + head0) * g.dim + col;
+#pragma unroll
+    for (int h = 0; h < kReadHeads; ++h) {
+        if (head0 + h >= g.heads) break;
+        const float s = __uint_as_float(b[h] << 23);
+        bf16x2 y[4] = {};
+        y[0] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(code[h], s, 0);
+        y[1] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(code[h], s, 1);
+        if constexpr (E == 8) {
+            y[2] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(code[h], s, 2);
+            y[3] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(code[h], s, 3);
+        }
+        float x[E];
+#pragma unroll
+        for (uint32_t j = 0; j < E; ++j) x[j] = b[h] == kKvScaleNaN ? __uint_as_float(0x7FC00000u) : (float)y[j / 2][j % 2];
+        kv_store16(out + (uint64_t)h * g.dim, x);
+    }
 }
 
 template <class T>
 static void launch_append(uint8_t *cache, const KvGeom &g, const void *k, uint64_t ks, const void *v, uint64_t vs, const uint64_t *slots, uint32_t n, hipStream_t s) {
     const T *kk = static_cast<const T *>(k), *vv = static_cast<const T *>(v);
     const uint32_t w = kv_width(g.dim), rows = 256 / (w / 8);
-    const dim3 grid((uint32_t)(((uint64_t)n + rows - 1) / rows * g.heads), 2);
+    const dim3 grid((uint32_t)(((uint64_t)n + rows - 1) / rows * ((g.heads + kAppendHeads - 1) / kAppendHeads)), 2);
     if (w == 64) hipLaunchKernelGGL((k_kv_append<T, 2>), grid, dim3(256), 0, s, cache, g, kk, ks, vv, vs, slots, n);
     else if (w == 128) hipLaunchKernelGGL((k_kv_append<T, 4>), grid, dim3(256), 0, s, cache, g, kk, ks, vv, vs, slots, n);
     else hipLaunchKernelGGL((k_kv_append<T, 8>), grid, dim3(256), 0, s, cache, g, kk, ks, vv, vs, slots, n);
@@ -343,8 +364,8 @@ static void launch_append(uint8_t *cache, const KvGeom &g, const void *k, uint64
 template <class T>
 static void launch_read(const uint8_t *cache, const KvGeom &g, const uint64_t *slots, uint32_t n, void *k, void *v, hipStream_t s) {
     T *kk = static_cast<T *>(k), *vv = static_cast<T *>(v);
-    const uint32_t w = kv_width(g.dim), rows = 256 / (w / 8);
-    const dim3 grid((uint32_t)(((uint64_t)n + rows - 1) / rows * g.heads), k && v ? 2 : 1);
+    const uint32_t w = kv_width(g.dim), rows = 256 * 16 / sizeof(T) / w, groups = (g.heads + kReadHeads - 1) / kReadHeads;
+    const dim3 grid((uint32_t)(((uint64_t)n + rows - 1) / rows * groups), k && v ? 2 : 1);
     if (w == 64) hipLaunchKernelGGL((k_kv_read<T, 2>), grid, dim3(256), 0, s, cache, g, slots, n, kk, vv);
     else if (w == 128) hipLaunchKernelGGL((k_kv_read<T, 4>), grid, dim3(256), 0, s, cache, g, slots, n, kk, vv);
     else hipLaunchKernelGGL((k_kv_read<T, 8>), grid, dim3(256), 0, s, cache, g, slots, n, kk, vv);
