@@ -289,7 +289,7 @@ def check_attend(torch, lengths, new, d, heads, group, page, kind, causal, seed=
         j = r - starts[i]
         return slice(0, max(0, lengths[i] - new[i] + j + 1) if causal else lengths[i])
 
-    pick = range(rows) if few is None or rows <= few else sorted(set(rng.choice(rows, few, replace=False)) | {0, rows - 1})
+    pick = range(rows) if few is None or rows <= few else sorted(set(rng.choice(rows, few, replace=False)) | {r for i, x in enumerate(new) if x for r in (starts[i], starts[i + 1] - 1)})
     check_rows(mem, got, lse, qx, [(r, owner[r]) for r in pick], group, kind, float(np.float32(scale)), visible)
     assert (got[rows:] == 77.0).all() and (lse[rows:] == 77.0).all()  # rows behind the last are left as they were
     return mem, q, got, lse, size
@@ -342,6 +342,20 @@ def test_prompts(torch, kind, causal, d, heads, group, page):
 @pytest.mark.parametrize("d", [64, 128, 256])
 def test_prompts_of_many_rows(torch, kind, d):
     check_attend(torch, [700, 333], [513, 200], d, 1, 3, 16, kind, True, few=40)
+
+
+@pytest.mark.parametrize("kind", ["bf16", "fp32"])
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("lengths,new,d,heads,group", [
+    ([900, 260, 0, 400, 311, 30], [300, 260, 0, 17, 290, 47], 64, 16, 2),             # rows that see nothing, requests of no row
+    ([513, 700, 1500, 641, 600], [500, 641, 64, 641, 333], 128, 16, 2),
+    ([5 * i % 97 + 60 for i in range(64)], [7 * i % 61 + 1 for i in range(64)], 64, 4, 3),
+    ([5 * i % 97 + 60 for i in range(65)], [7 * i % 61 + 1 for i in range(65)], 64, 4, 3),
+    ([400, 333], [300, 333], 256, 32, 2)])
+def test_prompts_of_more_blocks_than_the_card_has_units(torch, kind, causal, lengths, new, d, heads, group):
+    *_, got, lse, size = check_attend(torch, lengths, new, d, heads, group, 16, kind, causal, few=12)
+    rows = sum(new)
+    assert size == 0 and (got[:rows] != 77.0).all() and (lse[:rows] != 77.0).all()
 
 
 def test_rows_without_tokens_get_zero_and_minus_infinity(torch):

@@ -20,6 +20,7 @@
 // The maximum is lazy: m moves only when a score exceeds it by more than 2^kSlack (a wave-wide vote, no exchange between lanes);
 // exp2 arguments stay below kSlack, so sums of 2^31 tokens stay far inside fp32.
 #include "kv_cache.h"
+#include "wave_select.h"
 
 #include <algorithm>
 #include <cfloat>
@@ -39,7 +40,7 @@ struct KvAttendArgs {
     uint64_t q_stride;
     float scale_log2;  // scale * log2(e)
     uint32_t table_stride, group, n, rows, max_new, max_length, split_tokens, splits, tiles, k;
-    bool causal;
+    bool causal, longest_first;
 };
 
 constexpr float kSlack = 8.0f;
@@ -400,7 +401,7 @@ struct KvJoin {
 // What a block of k_kv_attend / k_kv_attend_wide works on: row tile x one key/value head x one split of the tokens of a request.  Blocks are
 // numbered head first, so that (with 8 heads) an XCD's L2 keeps the pages of its own heads, and row tiles last to first, so that the
 // causal ones with most tokens start first.  The requests turn by one from one tile or split to the next: blocks are dealt to the shader
-// engines in order, and without it one of them gets all of a long request (4 prompts: 465 -> 331 us).
+// engines in order, and without it one of them gets all of a long request (4 prompts, in the kernel's first form: 465 -> 331 us).
 struct KvWhere {  // what the block's number says: known before anything is read
     uint32_t head, i, split, tile;
     __device__ explicit KvWhere(const KvAttendArgs &a) {
@@ -411,6 +412,48 @@ struct KvWhere {  // what the block's number says: known before anything is read
         tile = a.tiles - 1 - turn / a.splits;
     }
 };
+
+// The same for up to 64 requests whose tiles are not split, where blocks are more than units: block b takes the b-th longest tile of all
+// requests, so that the last blocks to start are the shortest.  Each lane counts the tiles of one request that end behind some token, and
+// the token is searched for behind which no more than b of them end: some 2 us at a block's start, worth it where units get blocks one
+// after the other (4 prompts, 1,376 blocks: 245 us, 274 in turns; 2 requests of 197 x 16 rows at width 256, fp32, 400 blocks: 53, 85; 70
+// blocks of short prompts: 10.6, 10.1).  False: there is no such tile.  (All 64 lanes call this.)
+template <uint32_t ROWS>
+__device__ inline bool longest_first(const KvAttendArgs &a, KvWhere &where) {
+    const uint32_t lane = threadIdx.x & 63, rank = blockIdx.x / a.g.heads;
+    uint32_t tiles = 0, seeing = 0, reach = 0;  // row tiles, tokens whose rows these are, tokens that can be read
+    int64_t base = 0;
+    if (lane < a.n) {
+        const uint32_t first = min(a.starts[lane], a.rows), next = min(a.starts[lane + 1], a.rows), count = next > first ? next - first : 0, length = a.lengths[lane];
+        seeing = min(count, a.max_new);
+        tiles = (seeing * a.group + ROWS - 1) / ROWS;
+        reach = (uint32_t)min((uint64_t)min(length, a.max_length), (uint64_t)a.table_stride << a.g.page_shift);
+        base = (int64_t)length - count;
+    }
+    auto wave_sum = [&](uint32_t x) { return (uint32_t)__builtin_amdgcn_readlane((int)wave_incl_scan(x, (int)lane), 63); };
+    auto behind = [&](int32_t end) -> uint32_t {
+        if (end < 0) return tiles;
+        if ((uint32_t)end >= reach) return 0;
+        const int64_t x = end - base;  // the row of this token sees end + 1 of them, and is the first that does
+        if (!a.causal || x < 0) return tiles;
+        return x >= seeing ? 0 : tiles - (uint32_t)x * a.group / ROWS;
+    };
+    int32_t low = -1, high = (int32_t)a.max_length;
+    if (rank >= wave_sum(tiles)) return false;
+    while (high - low > 1) {
+        const int32_t mid = low + (high - low) / 2;
+        if (wave_sum(behind(mid)) > rank) low = mid;
+        else high = mid;
+    }
+    // of the tiles that end at `high`, in the order of the requests
+    const uint32_t longer = behind(high), here = behind(low) - longer;
+    const uint32_t upto = wave_incl_scan(here, (int)lane), skip = rank - wave_sum(longer), at = (uint32_t)__builtin_ctzll(__ballot(upto > skip));
+    where.i = at;
+    where.split = 0;
+    where.tile = (uint32_t)__builtin_amdgcn_readlane((int)(tiles - 1 - longer - (skip - (upto - here))), at);
+    return true;
+}
+
 struct KvBlock : KvWhere {
     uint32_t first, count, length, reach, rows, row0, end;
 
@@ -625,18 +668,19 @@ constexpr int wide_tiles(int nb, int terms) { return nb == 8 ? 1 : terms == 1 ? 
 // soon as it has widened the last, a whole chunk ahead.
 //
 // Bound by instruction issue: 32 tokens x 48 rows are 48 matrix instructions (768 cycles of the unit) and some 190 others, of which the
-// weights are two thirds; two waves on a SIMD overlap them in part.  4 prompts of 1,500 to 2,048 tokens, 32 heads, causal: 275 us, 0.90
-// PFLOP/s, where a library product of 8192^3 reaches 1.21.  Taken and measured: every wave widening for itself 331 us; 32 or 64 rows a
+// weights are two thirds; two waves on a SIMD overlap them in part.  4 prompts of 1,500 to 2,048 tokens, 32 heads, causal: 245 us, 1.02
+// PFLOP/s, where a library product of 8192^3 reaches 1.21.  Taken and measured (before the longest blocks came first, 275 us): every wave widening for itself 331 us; 32 or 64 rows a
 // wave 297 / 666 (registers); three waves of 32 rows on a SIMD 291; eight waves sharing a widened tile 300; raised priority around the
 // matrix instructions 308.  At width 256 a wave has 16 rows and the start and end of a block weigh as much as its 20 chunks (33 rows of 8
-// heads over 4,100 tokens: 51 us; two tiles a wave at one wave a SIMD 78; keys widened by every wave 86).
+// heads over 4,100 tokens: 49 us; two tiles a wave at one wave a SIMD 78; keys widened by every wave 86).
 template <int NB, int NT, int TERMS>
 __global__ __launch_bounds__(256, NB == 8 && TERMS == 3 ? 1 : 2) void k_kv_attend_wide(const KvAttendArgs a) {
     constexpr uint32_t TILES = NB == 8 ? 2 : 4, T = 16 * TILES;
     constexpr bool BOTH = NB < 8;  // a wave widens keys and values of its tile
     __shared__ uint4 keys[2][TILES][NB][64], vals[2][TILES / 2][2 * NB][64];
     const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4;
-    const KvWhere where(a);
+    KvWhere where(a);
+    if (a.longest_first && !longest_first<64 * NT>(a, where)) return;
     const uint32_t t0 = where.split * a.split_tokens;
     KvPages<T, T> pages(a, where.i, t0);
     const KvBlock blk(a, where, 64 * NT);
@@ -986,7 +1030,7 @@ __global__ __launch_bounds__(256, NB == 8 && TERMS == 3 ? 1 : NB == 8 || TERMS =
 // slowest (33 rows of 8 heads over 4,100 tokens: 52 us, 70 with two).  Few rows that leave units empty even so get eight waves to a
 // block (one request of 1,024 tokens: 9.0 us, 12.8 with four waves and splits).
 struct KvCut {
-    bool wide;
+    bool wide, longest_first;
     uint32_t nt, tiles, splits, split_tokens, waves;
     uint64_t blocks;
 };
@@ -1015,6 +1059,7 @@ static KvCut kv_cut(const KvGeom &g, uint32_t type, uint32_t group, uint32_t n, 
     c.split_tokens = (uint32_t)std::max<uint64_t>((((uint64_t)max_length + splits - 1) / splits + 127) / 128 * 128, 128);
     c.splits = (uint32_t)std::max<uint64_t>(((uint64_t)max_length + c.split_tokens - 1) / c.split_tokens, 1);
     c.blocks = base * c.splits;
+    c.longest_first = c.wide && c.splits == 1 && n > 1 && n <= 64 && c.blocks > (uint64_t)cus;
     c.waves = !c.wide && c.blocks <= (uint64_t)cus && w <= 128 && c.split_tokens > 256 ? 8 : 4;
     return c;
 }
@@ -1137,7 +1182,7 @@ int zvdb_hip_kv_attend_dev(const zvdb_hip_kv_layout *layout, const void *d_cache
     a.group = q_heads / a.g.heads;
     a.n = n; a.rows = rows; a.max_new = max_new; a.max_length = max_length;
     a.split_tokens = c.split_tokens; a.splits = c.splits; a.tiles = c.tiles;
-    a.causal = causal != 0;
+    a.causal = causal != 0; a.longest_first = c.longest_first;
     const uint32_t w = kv_width(a.g.dim);
     if (w == 64) launch_attend<2>(a, c, type, s);
     else if (w == 128) launch_attend<4>(a, c, type, s);
