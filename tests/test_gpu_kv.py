@@ -358,6 +358,18 @@ def test_prompts_of_more_blocks_than_the_card_has_units(torch, kind, causal, len
     assert size == 0 and (got[:rows] != 77.0).all() and (lse[:rows] != 77.0).all()
 
 
+@pytest.mark.parametrize("kind", ["bf16", "fp32"])
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("lengths,new,d,heads,group", [
+    ([1500, 40, 0, 900, 1211, 130], [100, 40, 3, 1, 61, 0], 64, 2, 3),
+    ([1100, 600, 1300, 20], [90, 2, 130, 47], 128, 4, 2),
+    ([1700, 310, 800], [40, 128, 3], 256, 4, 3)])
+def test_prompts_in_splits_of_more_blocks_than_units(torch, kind, causal, lengths, new, d, heads, group):
+    *_, got, lse, size = check_attend(torch, lengths, new, d, heads, group, 16, kind, causal, few=12)
+    rows = sum(new)
+    assert size > 0 and (got[:rows] != 77.0).all() and (lse[:rows] != 77.0).all()
+
+
 def test_rows_without_tokens_get_zero_and_minus_infinity(torch):
     for new in ([5, 1], [90, 2]):
         mem, q, got, lse, _ = check_attend(torch, [2, 0], new, 64, 1, 1, 16, "bf16", True)

@@ -40,7 +40,7 @@ struct KvAttendArgs {
     uint64_t q_stride;
     float scale_log2;  // scale * log2(e)
     uint32_t table_stride, group, n, rows, max_new, max_length, split_tokens, splits, tiles, k;
-    bool causal, longest_first;
+    bool causal, by_tile;
 };
 
 constexpr float kSlack = 8.0f;
@@ -413,13 +413,18 @@ struct KvWhere {  // what the block's number says: known before anything is read
     }
 };
 
-// The same for up to 64 requests whose tiles are not split, where blocks are more than units: block b takes the b-th longest tile of all
-// requests, so that the last blocks to start are the shortest.  Each lane counts the tiles of one request that end behind some token, and
-// the token is searched for behind which no more than b of them end: some 2 us at a block's start, worth it where units get blocks one
-// after the other (4 prompts, 1,376 blocks: 245 us, 274 in turns; 2 requests of 197 x 16 rows at width 256, fp32, 400 blocks: 53, 85; 70
-// blocks of short prompts: 10.6, 10.1).  False: there is no such tile.  (All 64 lanes call this.)
+// The same for up to 64 requests where blocks are more than units: the blocks of tiles that no request has come last instead of first, where
+// they held the units for some us before the others began.  False: there is no such tile.  (All 64 lanes call this.)
+//
+// Split tiles are numbered in the order of the requests, split by split (2 prompts of 1,329 x 4 rows, not causal: 30 us, 48 in turns; 313 x
+// 3 rows over 4,300 tokens: 26.5, 30.3; no difference where all requests have as many).
+//
+// Whole tiles go by length: block b takes the b-th longest of all requests, so that the last blocks to start are the shortest.  Each lane
+// counts the tiles of one request that end behind some token, and the token is searched for behind which no more than b of them end: some
+// 2 us at a block's start, worth it where units get blocks one after the other (4 prompts, 1,376 blocks: 245 us, 274 in turns; 2 requests of
+// 197 x 16 rows at width 256, fp32, 400 blocks: 53, 85; 70 blocks of short prompts: 10.6, 10.1).
 template <uint32_t ROWS>
-__device__ inline bool longest_first(const KvAttendArgs &a, KvWhere &where) {
+__device__ inline bool find_tile(const KvAttendArgs &a, KvWhere &where) {
     const uint32_t lane = threadIdx.x & 63, rank = blockIdx.x / a.g.heads;
     uint32_t tiles = 0, seeing = 0, reach = 0;  // row tiles, tokens whose rows these are, tokens that can be read
     int64_t base = 0;
@@ -429,6 +434,15 @@ __device__ inline bool longest_first(const KvAttendArgs &a, KvWhere &where) {
         tiles = (seeing * a.group + ROWS - 1) / ROWS;
         reach = (uint32_t)min((uint64_t)min(length, a.max_length), (uint64_t)a.table_stride << a.g.page_shift);
         base = (int64_t)length - count;
+    }
+    if (a.splits > 1) {
+        const uint32_t upto = wave_incl_scan(tiles, (int)lane), total = (uint32_t)__builtin_amdgcn_readlane((int)upto, 63);
+        if (rank >= (uint64_t)total * a.splits) return false;
+        const uint32_t nth = rank % total, at = (uint32_t)__builtin_ctzll(__ballot(upto > nth));
+        where.i = at;
+        where.split = rank / total;
+        where.tile = (uint32_t)__builtin_amdgcn_readlane((int)(nth - (upto - tiles)), at);
+        return true;
     }
     auto wave_sum = [&](uint32_t x) { return (uint32_t)__builtin_amdgcn_readlane((int)wave_incl_scan(x, (int)lane), 63); };
     auto behind = [&](int32_t end) -> uint32_t {
@@ -680,7 +694,7 @@ __global__ __launch_bounds__(256, NB == 8 && TERMS == 3 ? 1 : 2) void k_kv_atten
     __shared__ uint4 keys[2][TILES][NB][64], vals[2][TILES / 2][2 * NB][64];
     const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4;
     KvWhere where(a);
-    if (a.longest_first && !longest_first<64 * NT>(a, where)) return;
+    if (a.by_tile && !find_tile<64 * NT>(a, where)) return;
     const uint32_t t0 = where.split * a.split_tokens;
     KvPages<T, T> pages(a, where.i, t0);
     const KvBlock blk(a, where, 64 * NT);
@@ -1026,11 +1040,12 @@ __global__ __launch_bounds__(256, NB == 8 && TERMS == 3 ? 1 : NB == 8 || TERMS =
 // workspace and its place in the join, so parts have at least 1,024 tokens of few rows, 256 of many.  Few rows: four blocks for each unit
 // unless there are two (requests differ in length, a good third of the splits is empty: 48 requests to 8,192 tokens: 2 / 3 / 5 splits
 // 58.5 / 54.4 / 59.8 us; one of 32,768: 32 / 256 splits 15.5 / 28.9; 64 of 2,048: whole 29.8, two splits 39.8).  Many: none from one block
-// a unit on (7 prompts of 1,294 tokens, 294 blocks: 38 us, with four splits 82), else to two, four at width 256, whose blocks are the
-// slowest (33 rows of 8 heads over 4,100 tokens: 52 us, 70 with two).  Few rows that leave units empty even so get eight waves to a
+// a unit on (7 prompts of 1,294 tokens, 294 blocks: 35 us, with four splits 82), else to two, four at width 256 with bf16 queries, whose
+// blocks are the slowest (33 rows of 8 heads over 4,100 tokens: 49 us, 65 with two, 66 with six; fp32, one block resident on a unit: 4
+// prompts of 422 x 5 rows over 1,415: 37 us, 48 with four).  Few rows that leave units empty even so get eight waves to a
 // block (one request of 1,024 tokens: 9.0 us, 12.8 with four waves and splits).
 struct KvCut {
-    bool wide, longest_first;
+    bool wide, by_tile;
     uint32_t nt, tiles, splits, split_tokens, waves;
     uint64_t blocks;
 };
@@ -1051,7 +1066,7 @@ static KvCut kv_cut(const KvGeom &g, uint32_t type, uint32_t group, uint32_t n, 
         c.nt = 1;
         base = cut_rows();
     }
-    const uint64_t want = (uint64_t)cus * (c.wide && w < 256 ? 2 : 4);
+    const uint64_t want = (uint64_t)cus * (c.wide && (w < 256 || type == ZVDB_KV_F32) ? 2 : 4);
     uint64_t splits = base && base < (c.wide ? 1 : 2) * (uint64_t)cus ? (want + base - 1) / base : 1;
     const uint32_t least = c.wide ? 256 : 1024;
     splits = std::min<uint64_t>(splits, ((uint64_t)max_length + least - 1) / least);
@@ -1059,7 +1074,7 @@ static KvCut kv_cut(const KvGeom &g, uint32_t type, uint32_t group, uint32_t n, 
     c.split_tokens = (uint32_t)std::max<uint64_t>((((uint64_t)max_length + splits - 1) / splits + 127) / 128 * 128, 128);
     c.splits = (uint32_t)std::max<uint64_t>(((uint64_t)max_length + c.split_tokens - 1) / c.split_tokens, 1);
     c.blocks = base * c.splits;
-    c.longest_first = c.wide && c.splits == 1 && n > 1 && n <= 64 && c.blocks > (uint64_t)cus;
+    c.by_tile = c.wide && n > 1 && n <= 64 && c.blocks > (uint64_t)cus;
     c.waves = !c.wide && c.blocks <= (uint64_t)cus && w <= 128 && c.split_tokens > 256 ? 8 : 4;
     return c;
 }
@@ -1182,7 +1197,7 @@ int zvdb_hip_kv_attend_dev(const zvdb_hip_kv_layout *layout, const void *d_cache
     a.group = q_heads / a.g.heads;
     a.n = n; a.rows = rows; a.max_new = max_new; a.max_length = max_length;
     a.split_tokens = c.split_tokens; a.splits = c.splits; a.tiles = c.tiles;
-    a.causal = causal != 0; a.longest_first = c.longest_first;
+    a.causal = causal != 0; a.by_tile = c.by_tile;
     const uint32_t w = kv_width(a.g.dim);
     if (w == 64) launch_attend<2>(a, c, type, s);
     else if (w == 128) launch_attend<4>(a, c, type, s);
