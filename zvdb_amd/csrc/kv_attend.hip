@@ -582,7 +582,7 @@ __device__ inline void store_rows(const KvAttendArgs &a, const KvBlock &blk, con
 
 // Few rows (decode): 16 of them to a block, whose waves take the chunks of the split's tokens in turn and are joined in LDS.  Each wave
 // widens what it loads, one chunk of 32 tokens ahead: 4.3 KB at width 128, three waves on a SIMD.  Bound by HBM: 48 requests to 8,192
-// tokens, 8 x 128, bf16: 223 MB in 54 us with the join, 53 with the loads alone and no arithmetic; with fp32 queries, whose products run
+// tokens, 8 x 128, bf16: 223 MB in 53 us with the join, as long with the loads alone and no arithmetic; with fp32 queries, whose products run
 // three times, by the instructions around them (3 requests to 131,072 tokens, 4 x 64: 88 MB in 35 us, 30 with the loads alone).  One
 // masked step serves whole and cut chunks: two copies of it took 232 registers for 128 and one wave less.
 template <int NB, int TERMS, int WAVES>
@@ -681,8 +681,8 @@ constexpr int wide_tiles(int nb, int terms) { return nb == 8 ? 1 : terms == 1 ? 
 // tokens (32) at a time into one of two buffers while the other is read, one barrier for each.  A wave's next raw rows are requested as
 // soon as it has widened the last, a whole chunk ahead.
 //
-// Bound by instruction issue: 32 tokens x 48 rows are 48 matrix instructions (768 cycles of the unit) and some 190 others, of which the
-// weights are two thirds; two waves on a SIMD overlap them in part.  4 prompts of 1,500 to 2,048 tokens, 32 heads, causal: 245 us, 1.02
+// Bound by instruction issue: 32 tokens x 48 rows are 48 matrix instructions (768 cycles of the unit) and some 180 others (1,020), of which
+// the weights are two thirds; a SIMD's two waves overlap them by half at best, and what is lost to waits is as much.  4 prompts of 1,500 to 2,048 tokens, 32 heads, causal: 245 us, 1.02
 // PFLOP/s, where a library product of 8192^3 reaches 1.21.  Taken and measured (before the longest blocks came first, 275 us): every wave widening for itself 331 us; 32 or 64 rows a
 // wave 297 / 666 (registers); three waves of 32 rows on a SIMD 291; eight waves sharing a widened tile 300; raised priority around the
 // matrix instructions 308.  At width 256 a wave has 16 rows and the start and end of a block weigh as much as its 20 chunks (33 rows of 8

@@ -1,6 +1,6 @@
 // kv_pages.hip -- the 4-bit key/value cache's pages: planning (block tables, slot map), writing rows, reading them back.
 //
-// All three are bound by latency when a decode step calls them (4.0, 2.7 and 2.7 us on the device for 64 tokens) and by HBM when a prompt
+// All three are bound by latency when a decode step calls them (3.9, 2.7 and 2.7 us on the device for 64 tokens) and by HBM when a prompt
 // does; none has arithmetic worth counting.
 #include "kv_cache.h"
 
