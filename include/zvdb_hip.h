@@ -484,7 +484,7 @@ int zvdb_hip_kv_plan_dev(const zvdb_hip_kv_layout *layout, const void *d_lengths
                          uint64_t slot_cap, void *d_out_lengths, void *d_out_cursor, void *d_status, void *stream);
 
 /* Writes the keys and values of n tokens ([kv_heads][head_dim] of `type`, k_stride / v_stride elements from one token to the next, a
- * multiple of 8) into their slots.  Tokens without a slot are skipped.  A slot may be named once in a call. */
+ * multiple of 8 below 2^40) into their slots.  Tokens without a slot are skipped.  A slot may be named once in a call. */
 int zvdb_hip_kv_append_dev(const zvdb_hip_kv_layout *layout, void *d_cache, const void *d_k, uint64_t k_stride, const void *d_v, uint64_t v_stride,
                            uint32_t type, uint32_t n, const void *d_slots, void *stream);
 
@@ -492,7 +492,7 @@ int zvdb_hip_kv_append_dev(const zvdb_hip_kv_layout *layout, void *d_cache, cons
 int zvdb_hip_kv_read_dev(const zvdb_hip_kv_layout *layout, const void *d_cache, const void *d_slots, uint32_t n, void *d_k, void *d_v, uint32_t type, void *stream);
 
 /* Attention of new tokens over their requests, o = softmax(scale q K^T) V with fp32 sums; 0 < scale <= 1e38.  d_q: [rows][q_heads][head_dim] of `type`,
- * q_stride elements from one token to the next (a multiple of 8); request i has the rows d_starts[i] .. d_starts[i + 1] (at most
+ * q_stride elements from one token to the next (a multiple of 8 below 2^40); request i has the rows d_starts[i] .. d_starts[i + 1] (at most
  * max_new of them; d_starts as zvdb_hip_kv_plan_dev writes it) and d_lengths[i] tokens (at most max_length), its new ones included.
  * Query head h reads key/value head h / (q_heads / kv_heads).  causal: the j-th of m new tokens sees the tokens before position
  * length - m + j + 1; else all of them.  d_out [rows][q_heads][head_dim] of `type`, d_lse fp32 [rows][q_heads] (log of the sum of

@@ -79,6 +79,14 @@ def test_selected_refuses(bad):
     refused(lambda: selected(layout(), **bad))
 
 
+@pytest.mark.parametrize("stride", [-128, -2**40, 2**40, 2**63, 2**64 - 8])
+def test_strides_that_wrap_are_refused(stride):
+    refused(lambda: append(layout(), ks=stride))
+    refused(lambda: append(layout(), vs=stride))
+    refused(lambda: attend(layout(), q_stride=stride))
+    refused(lambda: selected(layout(), q_stride=stride))
+
+
 def test_nothing_to_do_is_done_without_a_device():
     lay = layout()
     append(lay, n=0)

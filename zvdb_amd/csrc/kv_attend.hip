@@ -681,12 +681,13 @@ constexpr int wide_tiles(int nb, int terms) { return nb == 8 ? 1 : terms == 1 ? 
 // tokens (32) at a time into one of two buffers while the other is read, one barrier for each.  A wave's next raw rows are requested as
 // soon as it has widened the last, a whole chunk ahead.
 //
-// Bound by instruction issue: 32 tokens x 48 rows are 48 matrix instructions (768 cycles of the unit) and some 180 others (1,020), of which
-// the weights are two thirds; a SIMD's two waves overlap them by half at best, and what is lost to waits is as much.  4 prompts of 1,500 to 2,048 tokens, 32 heads, causal: 245 us, 1.02
-// PFLOP/s, where a library product of 8192^3 reaches 1.21.  Taken and measured (before the longest blocks came first, 275 us): every wave widening for itself 331 us; 32 or 64 rows a
-// wave 297 / 666 (registers); three waves of 32 rows on a SIMD 291; eight waves sharing a widened tile 300; raised priority around the
-// matrix instructions 308.  At width 256 a wave has 16 rows and the start and end of a block weigh as much as its 20 chunks (33 rows of 8
-// heads over 4,100 tokens: 49 us; two tiles a wave at one wave a SIMD 78; keys widened by every wave 86).
+// Bound by instruction issue: 32 tokens x 48 rows are 48 matrix instructions (768 cycles of the unit) and some 180 others (1,020), of
+// which the weights are two thirds; a SIMD's two waves overlap them by half at best, and what is lost to waits is as much.  4 prompts of
+// 1,500 to 2,048 tokens, 32 heads, causal: 245 us, 1.02 PFLOP/s, where a library product of 8192^3 reaches 1.21.  Taken and measured
+// (before the longest blocks came first, 275 us): every wave widening for itself 331 us; 32 or 64 rows a wave 297 / 666 (registers); three
+// waves of 32 rows on a SIMD 291; eight waves sharing a widened tile 300; raised priority around the matrix instructions 308.  At width
+// 256 a wave has 16 rows and the start and end of a block weigh as much as its 20 chunks (33 rows of 8 heads over 4,100 tokens: 49 us; two
+// tiles a wave at one wave a SIMD 78; keys widened by every wave 86).
 template <int NB, int NT, int TERMS>
 __global__ __launch_bounds__(256, NB == 8 && TERMS == 3 ? 1 : 2) void k_kv_attend_wide(const KvAttendArgs a) {
     constexpr uint32_t TILES = NB == 8 ? 2 : 4, T = 16 * TILES;
@@ -1113,7 +1114,7 @@ static void launch_selected(const KvAttendArgs &a, uint32_t blocks, uint32_t typ
 static int check_queries(const KvGeom &g, const void *q, uint64_t q_stride, uint32_t type, uint32_t q_heads, float scale, const void *out, const void *cache) {
     KV_ARG(q && out && cache, "null argument");
     KV_ARG(kv_aligned(q, 16) && kv_aligned(out, 16) && kv_aligned(cache, 16), "kv_attend: cache, q and out need 16-byte alignment");
-    KV_ARG(q_stride >= (uint64_t)q_heads * g.dim && q_stride % 8 == 0, "kv_attend: a token's stride is at least q_heads * head_dim and a multiple of 8");
+    KV_ARG(kv_stride_ok(q_stride, (uint64_t)q_heads * g.dim), "kv_attend: a token's stride is at least q_heads * head_dim, below 2^40 and a multiple of 8");
     KV_ARG(scale > 0.0f && scale <= 1e38f, "kv_attend: scale %g (positive, at most 1e38)", (double)scale);
     (void)type;
     return ZVDB_OK;

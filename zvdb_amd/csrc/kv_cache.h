@@ -48,6 +48,10 @@ class KvDevice {
         }                                 \
     } while (0)
 
+// Elements from one token's row to the next.  Far above any memory, far below where a row's offset wraps (a negative stride is refused)
+constexpr uint64_t kKvStrideEnd = 1ull << 40;
+inline bool kv_stride_ok(uint64_t stride, uint64_t row) { return stride >= row && stride < kKvStrideEnd && stride % 8 == 0; }
+
 inline bool kv_aligned(const void *p, uintptr_t a) { return reinterpret_cast<uintptr_t>(p) % a == 0; }
 
 #if defined(__HIPCC__)

@@ -434,7 +434,7 @@ int zvdb_hip_kv_append_dev(const zvdb_hip_kv_layout *layout, void *d_cache, cons
     KV_ARG((uint64_t)n * g.heads < 0x7FFFFFFFull, "kv_append: the call is too large (%u tokens)", n);
     KV_ARG(kv_aligned(d_cache, 16) && kv_aligned(d_k, 16) && kv_aligned(d_v, 16) && kv_aligned(d_slots, 8), "kv_append: cache, k and v need 16-byte alignment, slots 8");
     const uint64_t row = (uint64_t)g.heads * g.dim;
-    KV_ARG(k_stride >= row && v_stride >= row && k_stride % 8 == 0 && v_stride % 8 == 0, "kv_append: a token's stride is at least kv_heads * head_dim = %llu and a multiple of 8", (unsigned long long)row);
+    KV_ARG(kv_stride_ok(k_stride, row) && kv_stride_ok(v_stride, row), "kv_append: a token's stride is at least kv_heads * head_dim = %llu, below 2^40 and a multiple of 8", (unsigned long long)row);
     const hipStream_t s = static_cast<hipStream_t>(stream);
     KvDevice dev;
     ZV_CHECK(dev.enter(d_cache, s));
