@@ -806,3 +806,44 @@ def test_searching_an_index_and_attending_to_what_it_found(torch, mode):
             assert set(best.tolist()) == set(ids[h, i].tolist()) and counts[h, i] == k
             o, l, bo, bl = ref.attend_row(qx[i, h], mem.k[best, h], mem.v[best, h], 0.125, "fp32")
             assert (np.abs(got[i, h] - o) <= bo).all() and abs(gl[i, h] - l) <= bl
+
+
+@pytest.mark.parametrize("max_new,max_length,split", [(300, 700, False), (100, 1500, True)])
+def test_prompts_from_a_graph(torch, max_new, max_length, split):
+    """Prompts captured once; lengths and row starts change on the device between the replays, and with them which blocks have tiles."""
+    heads, group, d, n, page = (16, 2, 64, 6, 16) if not split else (2, 3, 64, 6, 16)
+    qh, rows = heads * group, 2 * max_new
+    mem = Memory(torch, np.random.default_rng(41), [max_length] * n, d, heads, page)
+    q, _ = as_type(torch, np.random.default_rng(42).standard_normal((rows, qh, d)), "bf16")
+    typ = kv_type("bf16")
+    size = mem.lay.attend_workspace(typ, qh, n, rows, max_new, max_length)
+    assert (size > 0) == split
+    ws = torch.full((max(size, 16),), 255, dtype=torch.uint8, device="cuda")
+    tables, starts, lengths = mem.i32(mem.tables), mem.i32([0] * (n + 1)), mem.i32([0] * n)
+    out, lse = torch.empty((rows, qh, d), dtype=torch.bfloat16, device="cuda"), torch.empty((rows, qh), device="cuda")
+
+    def call():
+        mem.lay.attend_dev(mem.cache.data_ptr(), q.data_ptr(), qh * d, typ, qh, n, starts.data_ptr(), rows, max_new, lengths.data_ptr(), tables.data_ptr(),
+                           mem.stride, max_length, 0.125, True, ws.data_ptr(), size, out.data_ptr(), lse.data_ptr(), stream(torch))
+
+    warm = torch.cuda.Stream()
+    with torch.cuda.stream(warm):
+        call()
+    warm.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        call()
+    rng = np.random.default_rng(43)
+    for new in ([max_new, 0, 17, 1, 90, 30], [0] * n, [1] * n, [5, max_new, 60, 0, 0, max_new // 2], [64, 64, 0, 65, 63, 1]):
+        starts.copy_(mem.i32(np.concatenate(([0], np.cumsum(new)))))
+        lengths.copy_(mem.i32([x + int(rng.integers(0, max_length - x + 1)) for x in new]))
+        out.fill_(77.0), lse.fill_(77.0)
+        call()
+        torch.cuda.synchronize()
+        want = out.clone(), lse.clone()
+        assert (want[0][:sum(new)] != 77.0).all() and (want[0][sum(new):] == 77.0).all() and torch.isfinite(want[1][:sum(new)]).all()
+        for _ in range(3):
+            out.fill_(77.0), lse.fill_(77.0), ws.fill_(255)
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(out, want[0]) and torch.equal(lse, want[1])
