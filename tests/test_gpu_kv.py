@@ -351,6 +351,7 @@ def test_prompts_of_many_rows(torch, kind, d):
     ([513, 700, 1500, 641, 600], [500, 641, 64, 641, 333], 128, 16, 2),
     ([5 * i % 97 + 60 for i in range(64)], [7 * i % 61 + 1 for i in range(64)], 64, 4, 3),
     ([5 * i % 97 + 60 for i in range(65)], [7 * i % 61 + 1 for i in range(65)], 64, 4, 3),
+    ([900], [400], 104, 64, 2), ([700, 650], [300, 290], 128, 40, 2), ([700, 300], [300, 300], 56, 40, 2),  # two tiles to a wave
     ([400, 333], [300, 333], 256, 32, 2)])
 def test_prompts_of_more_blocks_than_the_card_has_units(torch, kind, causal, lengths, new, d, heads, group):
     *_, got, lse, size = check_attend(torch, lengths, new, d, heads, group, 16, kind, causal, few=12)

@@ -673,8 +673,9 @@ __global__ __launch_bounds__(64 * WAVES, NB == 8 && TERMS == 3 ? 1 : NB == 8 || 
     });
 }
 
-// Row tiles of a wave of k_kv_attend_wide: what 256 registers hold
-constexpr int wide_tiles(int nb, int terms) { return nb == 8 ? 1 : terms == 1 ? 3 : 2; }
+// Row tiles of a wave of k_kv_attend_wide, at most: what 256 registers hold, and at width 64 two, which leave room for more waves on a SIMD
+// (8 prompts of up to 1,000 tokens, 32 heads x 64: 30 us, 35 with three; fp32, 3 of up to 1,469: 93, 86 with three, but 4 of 2,048: 151, 185)
+constexpr int wide_tiles(int nb, int terms) { return nb == 8 ? 1 : nb == 4 && terms == 1 ? 3 : 2; }
 
 // Many rows (prompts): each of a block's four waves has NT tiles of its own and all walk the same tokens.  A wave's tile of 16 tokens (at
 // width 256 its keys or its values) is widened once for the block into LDS, in the order in which the matrix instructions take it: 64
@@ -1034,8 +1035,9 @@ __global__ __launch_bounds__(256, NB == 8 && TERMS == 3 ? 1 : NB == 8 || TERMS =
 // ---- launches -----------------------------------------------------------------------------------------------------------
 
 // How a call is cut.  Rows of one (request, head) that fit 64 are few: blocks of 16 whose waves divide the tokens; more of them give
-// each wave its own tiles, several where that makes two blocks for each unit of the card, else one (82 new tokens of 7 heads over 2,452:
-// 21.4 -> 14.6 us).
+// each wave its own tiles, as many as leave three blocks with rows for two units of the card (one prompt of 4,000 over 4,000, 16 heads: 218
+// us with two tiles, 264 with one, 258 with three; 8 prompts of up to 300 x 4 rows: 33 with one, 50 with three; 82 new tokens of 7 heads
+// over 2,452: 14.6 with one, 21.4 with three).  The total of the rows says how many blocks that is, where prompts are of many lengths.
 //
 // Tokens are split where blocks are fewer than the card wants.  Each part costs its start (some 5 us of dependent reads), its rows in the
 // workspace and its place in the join, so parts have at least 1,024 tokens of few rows, 256 of many.  Few rows: four blocks for each unit
@@ -1051,7 +1053,7 @@ struct KvCut {
     uint64_t blocks;
 };
 
-static KvCut kv_cut(const KvGeom &g, uint32_t type, uint32_t group, uint32_t n, uint32_t max_new, uint32_t max_length, int cus) {
+static KvCut kv_cut(const KvGeom &g, uint32_t type, uint32_t group, uint32_t n, uint32_t all_rows, uint32_t max_new, uint32_t max_length, int cus) {
     KvCut c;
     const uint64_t rows = (uint64_t)max_new * group;
     const uint32_t w = kv_width(g.dim);
@@ -1063,8 +1065,10 @@ static KvCut kv_cut(const KvGeom &g, uint32_t type, uint32_t group, uint32_t n, 
         return (uint64_t)g.heads * n * c.tiles;
     };
     uint64_t base = cut_rows();
-    if (c.nt > 1 && base < 2 * (uint64_t)cus) {
-        c.nt = 1;
+    // blocks that have rows, at most: the host knows how many rows there are in all
+    auto busy = [&]() { return std::min(base, (uint64_t)g.heads * ((uint64_t)all_rows * group / (64 * c.nt) + n)); };
+    while (c.nt > 1 && busy() < 3 * (uint64_t)cus / 2) {
+        --c.nt;
         base = cut_rows();
     }
     const uint64_t want = (uint64_t)cus * (c.wide && (w < 256 || type == ZVDB_KV_F32) ? 2 : 4);
@@ -1083,7 +1087,8 @@ static KvCut kv_cut(const KvGeom &g, uint32_t type, uint32_t group, uint32_t n, 
 template <int NB, int TERMS>
 static void launch_attend_as(const KvAttendArgs &a, const KvCut &c, hipStream_t s) {
     const dim3 grid((uint32_t)c.blocks), block(64 * c.waves);
-    if (c.wide && c.nt > 1) hipLaunchKernelGGL((k_kv_attend_wide<NB, wide_tiles(NB, TERMS), TERMS>), grid, block, 0, s, a);
+    if (c.wide && c.nt == 3) hipLaunchKernelGGL((k_kv_attend_wide<NB, wide_tiles(NB, TERMS), TERMS>), grid, block, 0, s, a);
+    else if (c.wide && c.nt == 2) hipLaunchKernelGGL((k_kv_attend_wide<NB, NB == 8 ? 1 : 2, TERMS>), grid, block, 0, s, a);
     else if (c.wide) hipLaunchKernelGGL((k_kv_attend_wide<NB, 1, TERMS>), grid, block, 0, s, a);
     else if (c.waves == 8) hipLaunchKernelGGL((k_kv_attend<NB < 8 ? NB : 4, TERMS, 8>), grid, block, 0, s, a);
     else hipLaunchKernelGGL((k_kv_attend<NB, TERMS, 4>), grid, block, 0, s, a);
@@ -1160,7 +1165,7 @@ int zvdb_hip_kv_attend_workspace(const zvdb_hip_kv_layout *layout, uint32_t type
     ZV_CHECK(attend_shape(g, type, q_heads, n, rows, max_new, max_length));
     int cus = 0;
     ZV_CHECK(device_cus(&cus));
-    const KvCut c = kv_cut(g, type, q_heads / g.heads, n, std::min(max_new, rows), max_length, cus);
+    const KvCut c = kv_cut(g, type, q_heads / g.heads, n, rows, std::min(max_new, rows), max_length, cus);
     *out_bytes = c.splits > 1 ? (uint64_t)rows * q_heads * c.splits * (g.dim + 4) * 4 : 0;
     return ZVDB_OK;
 }
@@ -1179,7 +1184,7 @@ int zvdb_hip_kv_attend_dev(const zvdb_hip_kv_layout *layout, const void *d_cache
     const hipStream_t s = static_cast<hipStream_t>(stream);
     KvDevice dev;
     ZV_CHECK(dev.enter(d_cache, s));
-    const KvCut c = kv_cut(a.g, type, q_heads / a.g.heads, n, max_new, max_length, dev.cus());
+    const KvCut c = kv_cut(a.g, type, q_heads / a.g.heads, n, rows, max_new, max_length, dev.cus());
     KV_ARG(c.blocks < 0x7FFFFFFFull, "kv_attend: the call is too large (%llu blocks)", (unsigned long long)c.blocks);
     const uint64_t need = c.splits > 1 ? (uint64_t)rows * q_heads * c.splits * (a.g.dim + 4) * 4 : 0;
     KV_ARG(workspace_bytes >= need && (need == 0 || (d_workspace && kv_aligned(d_workspace, 16))), "kv_attend: workspace %llu bytes, need %llu, 16-byte aligned",
