@@ -1040,13 +1040,15 @@ __global__ __launch_bounds__(256, NB == 8 && TERMS == 3 ? 1 : NB == 8 || TERMS =
 // over 2,452: 14.6 with one, 21.4 with three).  The total of the rows says how many blocks that is, where prompts are of many lengths.
 //
 // Tokens are split where blocks are fewer than the card wants.  Each part costs its start (some 5 us of dependent reads), its rows in the
-// workspace and its place in the join, so parts have at least 1,024 tokens of few rows, 256 of many.  Few rows: four blocks for each unit
-// unless there are two (requests differ in length, a good third of the splits is empty: 48 requests to 8,192 tokens: 2 / 3 / 5 splits
-// 58.5 / 54.4 / 59.8 us; one of 32,768: 32 / 256 splits 15.5 / 28.9; 64 of 2,048: whole 29.8, two splits 39.8).  Many: none from one block
-// a unit on (7 prompts of 1,294 tokens, 294 blocks: 35 us, with four splits 82), else to two, four at width 256 with bf16 queries, whose
-// blocks are the slowest (33 rows of 8 heads over 4,100 tokens: 49 us, 65 with two, 66 with six; fp32, one block resident on a unit: 4
-// prompts of 422 x 5 rows over 1,415: 37 us, 48 with four).  Few rows that leave units empty even so get eight waves to a
-// block (one request of 1,024 tokens: 9.0 us, 12.8 with four waves and splits).
+// workspace and its place in the join.  Few rows: none up to 1,024 tokens (one request: 9.2 us, 11.6 in two), parts of at least 512 up to
+// 32 parts (16 requests to 4,000, fp32: 18 us, 23 with 1,024), of 1,024 beyond (one head over 131,072: 18 us, 22 with 512), up to four
+// blocks for each unit unless there are two (requests differ in length, a good third of the splits is empty: 48 requests to 8,192 tokens:
+// 2 / 3 / 5 splits 58.5 / 53.4 / 59.8 us; 64 of 2,048: whole 29.8, two splits 39.8); at width 256, where a unit holds one block or two, up
+// to one (24 requests to 11,000, fp32: 35 us, 43 with four; 64 to 2,000: 22, 25).  Many: none from one block a unit on (7 prompts of 1,294
+// tokens, 294 blocks: 35 us, with four splits 82), else to two, four at width 256 with bf16 queries, whose blocks are the slowest (33 rows
+// of 8 heads over 4,100 tokens: 49 us, 65 with two, 66 with six; fp32, one block resident on a unit: 4 prompts of 422 x 5 rows over 1,415:
+// 37 us, 48 with four).  Few rows that leave units empty even so get eight waves to a block (one request of 1,024 tokens: 9.0 us, 12.8 with
+// four waves and splits).
 struct KvCut {
     bool wide, by_tile;
     uint32_t nt, tiles, splits, split_tokens, waves;
@@ -1071,10 +1073,10 @@ static KvCut kv_cut(const KvGeom &g, uint32_t type, uint32_t group, uint32_t n, 
         --c.nt;
         base = cut_rows();
     }
-    const uint64_t want = (uint64_t)cus * (c.wide && (w < 256 || type == ZVDB_KV_F32) ? 2 : 4);
-    uint64_t splits = base && base < (c.wide ? 1 : 2) * (uint64_t)cus ? (want + base - 1) / base : 1;
-    const uint32_t least = c.wide ? 256 : 1024;
-    splits = std::min<uint64_t>(splits, ((uint64_t)max_length + least - 1) / least);
+    const uint64_t want = (uint64_t)cus * (c.wide ? (w < 256 || type == ZVDB_KV_F32 ? 2 : 4) : w < 256 ? 4 : 1);
+    uint64_t splits = base && base < (c.wide || w == 256 ? 1 : 2) * (uint64_t)cus ? (want + base - 1) / base : 1;
+    auto parts_of = [&](uint64_t tokens) { return (max_length + tokens - 1) / tokens; };
+    splits = std::min<uint64_t>(splits, c.wide ? parts_of(256) : max_length <= 1024 ? 1 : std::max<uint64_t>(std::min<uint64_t>(parts_of(512), 32), parts_of(1024)));
     splits = std::max<uint64_t>(std::min<uint64_t>(splits, 256), 1);
     c.split_tokens = (uint32_t)std::max<uint64_t>((((uint64_t)max_length + splits - 1) / splits + 127) / 128 * 128, 128);
     c.splits = (uint32_t)std::max<uint64_t>(((uint64_t)max_length + c.split_tokens - 1) / c.split_tokens, 1);
