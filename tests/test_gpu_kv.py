@@ -411,6 +411,49 @@ def test_a_nan_reaches_the_rows_that_see_it_and_no_others(torch, kind, d):
     check_attend(torch, [50], [40], d, 1, 2, 16, kind, False, spoil=lambda mem, k, v: v.__setitem__((30, 0, 33), np.nan))
 
 
+def loud_key(mem, k, request, token, head=slice(None)):
+    """Queries of check_loud have 8 in element 0, where only this token's key is not 0: it scores hundreds above all others."""
+    k[mem.first[request] + token, head, 0] = 1000.0
+
+
+def check_loud(torch, lengths, new, d, heads, group, kind, causal, spoil, few=None, **kw):
+    """As check_attend, with queries that meet loud_key."""
+    rng = np.random.default_rng(d + sum(lengths))
+
+    def all_of_it(mem, k, v):
+        k[:, :, 0] = 0.0
+        spoil(mem, k, v)
+
+    with np.errstate(invalid="ignore"):
+        mem = Memory(torch, rng, lengths, d, heads, 16, spoil=all_of_it)
+    x = rng.standard_normal((sum(new), heads * group, d))
+    x[:, :, 0] = 8.0
+    q, qx = as_type(torch, x, kind)
+    scale, starts = 1.0 / np.sqrt(d), np.concatenate(([0], np.cumsum(new))).astype(int)
+    got, lse, size = attend(mem, q, new, group, kind, causal, scale, **kw)
+    owner = np.repeat(np.arange(len(new)), new)
+    pick = range(sum(new)) if few is None or sum(new) <= few else sorted(set(rng.choice(sum(new), few, replace=False)) | set(starts[:-1]) | set(starts[1:] - 1))
+    check_rows(mem, got, lse, qx, [(r, owner[r]) for r in pick], group, kind, float(np.float32(scale)),
+               lambda r, i: slice(0, lengths[i] - new[i] + r - starts[i] + 1 if causal else lengths[i]))
+    return got, size
+
+
+@pytest.mark.parametrize("kind", ["bf16", "fp32"])
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("new,bound", [([1, 1, 1], 4096), ([1, 1, 1], 4608), ([60, 1, 33], 2500)])  # eight splits, nine, prompts
+def test_a_nan_is_kept_where_its_split_weighs_nothing(torch, kind, d, new, bound):
+    """One key outweighs every other split of its request by more than fp32 can hold; the NaN of a value lies in another one, before or
+    behind it, and reaches the rows all the same: 0 NaN is NaN."""
+    def spoil(mem, k, v):
+        loud_key(mem, k, 0, 10), loud_key(mem, k, 1, 2040)
+        v[mem.first[0] + 2300, 0, 3] = np.nan
+        v[mem.first[1] + 5, 1, d - 1] = np.inf
+        v[mem.first[1] + 700, 0, 0] = -np.inf
+
+    got, size = check_loud(torch, [2400, 2100, 90], new, d, 2, 2, kind, True, spoil, few=8, max_length=bound)
+    assert size > 0 and np.isnan(got[0]).any() and np.isnan(got[new[0]]).any()
+
+
 def test_scores_of_any_size(torch):
     """Large scores, rows whose maximum moves late, all scores equal, all far below zero."""
     def spoil(mem, k, v):

@@ -856,9 +856,9 @@ __global__ __launch_bounds__(256) void k_kv_join_few(const KvAttendArgs a, uint3
     for (uint32_t u = 0; u < kFewSplits; ++u) {
         if (u >= a.splits) break;
         if (ml[u].x == -INFINITY) continue;  // (the split saw nothing and left nothing)
-        const float by = __builtin_amdgcn_exp2f(ml[u].x - m);
+        const float by = __builtin_amdgcn_exp2f(ml[u].x - m);  // 0 spares nothing: a NaN that the split holds stays one
         l += ml[u].y * by;
-        if (by != 0.0f) { o.x += x[u].x * by; o.y += x[u].y * by; o.z += x[u].z * by; o.w += x[u].w * by; }
+        o.x += x[u].x * by; o.y += x[u].y * by; o.z += x[u].z * by; o.w += x[u].w * by;
     }
     const bool some = m != -INFINITY;
     const float by = some ? 1.0f / l : 0.0f;
@@ -894,7 +894,7 @@ __global__ __launch_bounds__(256) void k_kv_join(const KvAttendArgs a) {
     if ((tid & 63) == 0) red[0][tid >> 6] = m;
     __syncthreads();
     m = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
-    const float w = ms == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ms - m);  // (-inf: the split saw nothing and left nothing)
+    const float w = ms == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ms - m);  // (-inf: the split saw nothing and left zeros)
     weight[tid] = w;
     float l = ms == -INFINITY ? 0.0f : ls * w;
 #pragma unroll
@@ -903,8 +903,8 @@ __global__ __launch_bounds__(256) void k_kv_join(const KvAttendArgs a) {
     __syncthreads();
     float4 o = make_float4(0, 0, 0, 0);
     auto add = [&](const float4 &x, uint32_t s) {
-        const float by = weight[s];
-        if (by != 0.0f) { o.x += x.x * by; o.y += x.y * by; o.z += x.z * by; o.w += x.w * by; }
+        const float by = weight[s];  // 0 spares nothing: a NaN that the split holds stays one
+        o.x += x.x * by; o.y += x.y * by; o.z += x.z * by; o.w += x.w * by;
     };
     if (mine) {
 #pragma unroll
