@@ -454,6 +454,56 @@ def test_a_nan_is_kept_where_its_split_weighs_nothing(torch, kind, d, new, bound
     assert size > 0 and np.isnan(got[0]).any() and np.isnan(got[new[0]]).any()
 
 
+def check_sizes(torch, lengths, new, d, heads, group, kind, causal, power=125, few=None, **kw):
+    """Values of 2^power -- a block holds up to 6 x 2^125 -- against scores that differ by less than the slack of a running maximum: what
+    a sum of exponentials times the largest comes to before it is divided does not fit fp32."""
+    def spoil(mem, k, v):
+        k[:] = 0.0
+        for i, t in enumerate(lengths):
+            k[mem.first[i] + t // 2:mem.first[i + 1], :, 0] = 4.0    # 4.5 more (6.5 as powers of two) in the second half
+            k[mem.first[i] + t - 1:mem.first[i + 1], :, 0] = 3.0
+        v[:, :, ::4] = np.abs(v[:, :, ::4]) * 2.0 ** power            # columns of one sign
+        v[:, :, 1::4] *= 2.0 ** power                                 # and of both
+        np.clip(v, -2.5e38, 2.5e38, out=v)
+
+    rng = np.random.default_rng(d + sum(lengths))
+    mem = Memory(torch, rng, lengths, d, heads, 16, spoil=spoil)
+    x = rng.standard_normal((sum(new), heads * group, d))
+    x[:, :, 0] = 4.5 * np.sqrt(d) / 4.0
+    q, qx = as_type(torch, x, kind)
+    scale, starts = 1.0 / np.sqrt(d), np.concatenate(([0], np.cumsum(new))).astype(int)
+    got, lse, size = attend(mem, q, new, group, kind, causal, scale, **kw)
+    owner = np.repeat(np.arange(len(new)), new)
+    pick = range(sum(new)) if few is None or sum(new) <= few else sorted(set(rng.choice(sum(new), few, replace=False)) | set(starts[:-1]) | set(starts[1:] - 1))
+    check_rows(mem, got, lse, qx, [(r, owner[r]) for r in pick], group, kind, float(np.float32(scale)),
+               lambda r, i: slice(0, lengths[i] - new[i] + r - starts[i] + 1 if causal else lengths[i]))
+    return mem, q, qx, size
+
+
+@pytest.mark.parametrize("kind", ["bf16", "fp32"])
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("lengths,new,bound,split", [
+    ([2, 33, 64, 100, 257, 1000], [1] * 6, 1000, False), ([2400, 700, 3], [1] * 3, 4096, True), ([2400, 700, 3], [1] * 3, 4608, True),  # single tokens
+    ([300, 130], [40, 129], 300, None), ([2100, 900], [60, 70], 2100, True)])                                                          # prompts
+def test_values_near_the_largest_stay_finite(torch, kind, d, lengths, new, bound, split):
+    *_, size = check_sizes(torch, lengths, new, d, 2, 2, kind, True, few=8, max_length=bound)
+    assert split is None or (size > 0) == split
+
+
+@pytest.mark.parametrize("kind", ["bf16", "fp32"])
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_small_values_keep_their_bits(torch, kind, d):
+    for new in ([1, 1], [60, 70]):
+        check_sizes(torch, [300, 2100], new, d, 2, 2, kind, True, power=-108, few=8)
+
+
+@pytest.mark.parametrize("kind", ["bf16", "fp32"])
+@pytest.mark.parametrize("d,heads", [(64, 16), (128, 16), (256, 32)])
+def test_values_near_the_largest_in_whole_prompts(torch, kind, d, heads):
+    *_, size = check_sizes(torch, [400, 700], [300, 290], d, heads, 2, kind, False, few=4)
+    assert size == 0
+
+
 def test_scores_of_any_size(torch):
     """Large scores, rows whose maximum moves late, all scores equal, all far below zero."""
     def spoil(mem, k, v):
@@ -638,6 +688,17 @@ def test_selected_rows_of_hidden_pages_and_nan(torch):
     q, qx = as_type(torch, rng.standard_normal((2, 4, 64)), "bf16")
     got, lse = selected(mem, q, ids, None, 2, "bf16", 0.3)
     check_selected(mem, got, lse, qx, ids, None, 2, "bf16", float(np.float32(0.3)), there=lambda i, t: not (i == 0 and t // 16 == 4))
+
+
+@pytest.mark.parametrize("kind", ["bf16", "fp32"])
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_selected_values_near_the_largest_stay_finite(torch, kind, d):
+    lengths = [300, 90]
+    mem, q, qx, _ = check_sizes(torch, lengths, [1, 1], d, 2, 2, kind, True)
+    ids = np.stack([np.stack([np.arange(300) % t for t in lengths]) for _ in range(2)]).astype(np.uint64)
+    scale = 1.0 / np.sqrt(d)
+    got, lse = selected(mem, q, ids, None, 2, kind, scale)
+    check_selected(mem, got, lse, qx, ids, None, 2, kind, float(np.float32(scale)))
 
 
 def test_lists_of_no_rows(torch):

@@ -17,8 +17,10 @@
 // P is of the unrounded values.  fp32 queries: q and P are split into three bf16 terms each (24 bits,
 // exact for q) and every product runs three times.
 //
-// The maximum is lazy: m moves only when a score exceeds it by more than 2^kSlack (a wave-wide vote, no exchange between lanes);
-// exp2 arguments stay below kSlack, so sums of 2^31 tokens stay far inside fp32.
+// The maximum is lazy: it moves only when a score exceeds it by more than kSlack (a wave-wide vote, no exchange between lanes).  m lies
+// `lift` = kSlack + log2(tokens) above it, so that no weight is over 1 / tokens and no sum of weights times values, in a wave, a split or a join, is over
+// the largest of the values: they go up to 6 x 2^125.  What it costs lies at the other end: products under 2^-126 lose bits, 2^(lift - 149) of
+// each in the result, which is 2^-128 over 8,192 tokens.
 #include "kv_cache.h"
 #include "wave_select.h"
 
@@ -39,11 +41,13 @@ struct KvAttendArgs {
     const uint32_t *counts;
     uint64_t q_stride;
     float scale_log2;  // scale * log2(e)
+    float lift;
     uint32_t table_stride, group, n, rows, max_new, max_length, split_tokens, splits, tiles, k;
     bool causal, by_tile;
 };
 
 constexpr float kSlack = 8.0f;
+inline float kv_lift(uint32_t tokens) { return kSlack + (tokens > 1 ? 32 - __builtin_clz(tokens - 1) : 0); }
 constexpr float kNone = -FLT_MAX;  // maximum of a row that has seen nothing: exp2(-inf - kNone) = 0, never NaN
 constexpr float kLn2 = 0.693147180559945309f;
 
@@ -210,7 +214,7 @@ struct KvRows {
     // Scores to weights.  `seen(t, i, j)`: whether this lane's row of row tile t sees token 4 g + j of token tile i; asked only where
     // `mask` (uniform).
     template <class Seen>
-    __device__ void weights(f32x4 (*s)[2], bf16x8 (*p)[TERMS], float scale_log2, bool mask, Seen seen) {
+    __device__ void weights(f32x4 (*s)[2], bf16x8 (*p)[TERMS], float scale_log2, float lift, bool mask, Seen seen) {
         if (mask) {
 #pragma unroll
             for (int t = 0; t < NT; ++t)
@@ -226,12 +230,12 @@ struct KvRows {
 #pragma unroll
             for (int j = 1; j < 8; ++j) mx[t] = fmaxf(mx[t], s[t][j / 4][j % 4]);
             mx[t] *= scale_log2;
-            over |= mx[t] > m[t] + kSlack;
+            over |= mx[t] > m[t] + (kSlack - lift);
         }
         if (__any(over)) {
 #pragma unroll
             for (int t = 0; t < NT; ++t) {
-                const float to = fmaxf(m[t], max_over_row(mx[t])), by = __builtin_amdgcn_exp2f(m[t] - to);
+                const float to = fmaxf(m[t], max_over_row(mx[t]) + lift), by = __builtin_amdgcn_exp2f(m[t] - to);
                 m[t] = to;
                 l[t] *= by;
 #pragma unroll
@@ -269,13 +273,13 @@ struct KvRows {
 
     // 32 tokens that this wave widens for itself; `token(i, j)`: the index that nan_at counts of token 4 g + j of token tile i
     template <class Seen, class Token>
-    __device__ void step(const KvRaw<NB> &raw, float scale_log2, bool mask, Seen seen, Token token) {
+    __device__ void step(const KvRaw<NB> &raw, float scale_log2, float lift, bool mask, Seen seen, Token token) {
         float vs[8];
         nan_at = min(nan_at, value_scales<2>(raw.vs, vs, token));
         f32x4 s[NT][2];
         scores(s, [&](int i, int b) { return widen_key(raw.k[i][b], pow2_of(raw.ks[i], NB == 8 ? b / 4 : 0)); });
         bf16x8 p[NT][TERMS];
-        weights(s, p, scale_log2, mask, seen);
+        weights(s, p, scale_log2, lift, mask, seen);
         products(p, [&](int b, bf16x8 *a) {
             uint2 lo[2], hi[2];
             widen_values<NB>(raw.v[0], vs, b, lo[0], hi[0]);
@@ -630,7 +634,7 @@ __global__ __launch_bounds__(64 * WAVES, NB == 8 && TERMS == 3 ? 1 : NB == 8 || 
 #pragma unroll
                 for (int x = 0; x < 2; ++x) raw.vs[x] &= live_scales(there >> x & 1, t + 16 * x + 4 * g, t1);
             }
-            r.step(raw, a.scale_log2, part || t + 32 > all_see,
+            r.step(raw, a.scale_log2, a.lift, part || t + 32 > all_see,
                    [&](int, int x, int j) { const uint32_t at = t + 16 * x + 4 * g + j; return (there >> x & 1) && at < limit && at < t1; },
                    [&](int x, int j) { return t + 16 * x + 4 * g + j; });
         };
@@ -778,7 +782,7 @@ __global__ __launch_bounds__(256, NB == 8 && TERMS == 3 ? 1 : 2) void k_kv_atten
                 f32x4 s[NT][2];
                 r.scores(s, [&](int x, int b) { return __builtin_bit_cast(bf16x8, keys[buf][2 * h + x][b][lane]); });
                 bf16x8 p[NT][TERMS];
-                r.weights(s, p, a.scale_log2, !(here[0] && here[1]) || th + 32 > all_see || th + 32 > t1,
+                r.weights(s, p, a.scale_log2, a.lift, !(here[0] && here[1]) || th + 32 > all_see || th + 32 > t1,
                           [&](int row_tile, int x, int j) { const uint32_t at = th + 16 * x + 4 * g + j; return here[x] && at < limit[row_tile] && at < t1; });
                 r.products(p, [&](int b, bf16x8 *v2) {
                     v2[0] = __builtin_bit_cast(bf16x8, vals[buf][h][2 * b][lane]);
@@ -1015,7 +1019,7 @@ __global__ __launch_bounds__(256, NB == 8 && TERMS == 3 ? 1 : NB == 8 || TERMS =
                 }
             }
             any |= seen != 0;
-            r.step(raw, a.scale_log2, true, [&](int, int x, int j) { return seen >> (4 * x + j) & 1; }, [](int, int) { return 0u; });
+            r.step(raw, a.scale_log2, a.lift, true, [&](int, int x, int j) { return seen >> (4 * x + j) & 1; }, [](int, int) { return 0u; });
         }
     }
     r.close();
@@ -1203,6 +1207,7 @@ int zvdb_hip_kv_attend_dev(const zvdb_hip_kv_layout *layout, const void *d_cache
     a.scale_log2 = scale * 1.44269504088896341f;
     a.table_stride = table_stride;
     a.group = q_heads / a.g.heads;
+    a.lift = kv_lift(max_length);
     a.n = n; a.rows = rows; a.max_new = max_new; a.max_length = max_length;
     a.split_tokens = c.split_tokens; a.splits = c.splits; a.tiles = c.tiles;
     a.causal = causal != 0; a.by_tile = c.by_tile;
@@ -1249,6 +1254,7 @@ int zvdb_hip_kv_attend_selected_dev(const zvdb_hip_kv_layout *layout, const void
     a.scale_log2 = scale * 1.44269504088896341f;
     a.table_stride = table_stride;
     a.group = q_heads / a.g.heads;
+    a.lift = kv_lift(k);
     a.n = n; a.k = k;
     const uint64_t blocks = (uint64_t)a.g.heads * n * ((a.group + 15) / 16);
     KV_ARG(blocks < 0x7FFFFFFFull, "kv_attend_selected: the call is too large (%llu blocks)", (unsigned long long)blocks);
