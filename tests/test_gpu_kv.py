@@ -498,6 +498,26 @@ def test_small_values_keep_their_bits(torch, kind, d):
 
 
 @pytest.mark.parametrize("kind", ["bf16", "fp32"])
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("length,new,heads", [(40, 1, 1), (2100, 1, 1), (40, 33, 2), (1500, 70, 2), (300, 280, 32)])
+def test_rows_whose_scores_are_all_minus_infinity(torch, kind, d, length, new, heads):
+    """Finite queries and keys whose products leave fp32 downwards: no token has a weight, as where none is seen."""
+    def spoil(mem, k, v):
+        k[:] = 0.0
+        k[:, :, 5] = 6.0
+
+    mem = Memory(torch, np.random.default_rng(d), [length], d, heads, 16, spoil=spoil)
+    q = torch.zeros((new, 2 * heads, d), dtype=torch.bfloat16 if kind == "bf16" else torch.float32, device="cuda")
+    q[:, :, 5] = -3e38
+    got, lse, _ = attend(mem, q, [new], 2, kind, True, 0.125)
+    assert (got[:new] == 0).all() and np.isneginf(lse[:new]).all()
+    if new == 1:
+        ids = np.tile(np.arange(length, dtype=np.uint64), (heads, 1, 1))
+        got, lse = selected(mem, q, ids, None, 2, kind, 0.125)
+        assert (got[:1] == 0).all() and np.isneginf(lse[:1]).all()
+
+
+@pytest.mark.parametrize("kind", ["bf16", "fp32"])
 @pytest.mark.parametrize("d,heads", [(64, 16), (128, 16), (256, 32)])
 def test_values_near_the_largest_in_whole_prompts(torch, kind, d, heads):
     *_, size = check_sizes(torch, [400, 700], [300, 290], d, heads, 2, kind, False, few=4)

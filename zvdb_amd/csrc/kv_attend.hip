@@ -349,6 +349,8 @@ __device__ inline uint32_t live_scales(bool there, uint32_t at, uint32_t t1) {
     return live == 4 ? ~0u : (1u << (8 * live)) - 1;
 }
 
+// 1 / l; 0 where nothing is seen, or no score above -inf (a NaN among them is in O already)
+__device__ inline float over_sum(float l) { return l > 0.0f ? 1.0f / l : 0.0f; }
 __device__ inline float lse_of(float m, float l) { return (m + __log2f(l)) * kLn2; }
 
 // Where the waves of a block that share 16 rows and have tokens of their own are joined: every wave leaves what it has, and after one
@@ -562,7 +564,7 @@ __device__ inline void store_rows(const KvAttendArgs &a, const KvBlock &blk, con
         if (row >= blk.rows) continue;
         const uint64_t at = blk.place(a, row);
         const bool some = seen_from < limit[t], whole = a.splits == 1;
-        const float by = whole ? (some ? 1.0f / r.l[t] : 0.0f) : 1.0f;
+        const float by = whole ? over_sum(r.l[t]) : 1.0f;
         float *part = a.part + (at * a.splits + blk.split) * (a.g.dim + 4);
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
@@ -661,7 +663,7 @@ __global__ __launch_bounds__(64 * WAVES, NB == 8 && TERMS == 3 ? 1 : NB == 8 || 
         const uint64_t at = blk.place(a, blk.row0 + row);
         const bool some = seen_from < blk.limit(a, blk.row0 + row);
         if (whole) {
-            const float by = some ? 1.0f / l : 0.0f;
+            const float by = over_sum(l);
 #pragma unroll
             for (int e = 0; e < 4; ++e) y[e] *= by;
             store_columns<2, TERMS>(static_cast<uint8_t *>(a.out) + at * a.g.dim * (TERMS == 1 ? 2 : 4), d, a.g.dim, y);
@@ -865,7 +867,7 @@ __global__ __launch_bounds__(256) void k_kv_join_few(const KvAttendArgs a, uint3
         o.x += x[u].x * by; o.y += x[u].y * by; o.z += x[u].z * by; o.w += x[u].w * by;
     }
     const bool some = m != -INFINITY;
-    const float by = some ? 1.0f / l : 0.0f;
+    const float by = over_sum(l);
     const float y[4] = {o.x * by, o.y * by, o.z * by, o.w * by};
     constexpr uint32_t kSize = TERMS == 1 ? 2 : 4;
     store_columns<2, TERMS>(static_cast<uint8_t *>(a.out) + row * a.g.dim * kSize, d, a.g.dim, y);
@@ -927,7 +929,7 @@ __global__ __launch_bounds__(256) void k_kv_join(const KvAttendArgs a) {
     }
     l = (red[1][0] + red[1][1]) + (red[1][2] + red[1][3]);
     const bool some = m != -INFINITY;
-    const float by = some ? 1.0f / l : 0.0f;
+    const float by = over_sum(l);
     const float y[4] = {o.x * by, o.y * by, o.z * by, o.w * by};
     constexpr uint32_t kSize = TERMS == 1 ? 2 : 4;
     if (mine) store_columns<2, TERMS>(static_cast<uint8_t *>(a.out) + row * a.g.dim * kSize, d, a.g.dim, y);
@@ -1028,7 +1030,7 @@ __global__ __launch_bounds__(256, NB == 8 && TERMS == 3 ? 1 : NB == 8 || TERMS =
     lds.join.leave(r, rows, waves ? waves : 1, 1);
     lds.join.take(rows, waves ? waves : 1, a.g.dim, [&](uint32_t at, uint32_t d, float *y, float m, float l) {
         const uint64_t out_row = (uint64_t)i * qheads + head * a.group + tile * 16 + at;
-        const float by = some ? 1.0f / l : 0.0f;
+        const float by = over_sum(l);
 #pragma unroll
         for (int e = 0; e < 4; ++e) y[e] *= by;
         store_columns<2, TERMS>(static_cast<uint8_t *>(a.out) + out_row * a.g.dim * kSize, d, a.g.dim, y);
