@@ -743,6 +743,92 @@ def test_selecting_every_row_is_attending_to_all(torch):
             assert (np.abs(got[i, h] - want[i, h]) <= 2 * bo).all() and abs(lse[i, h] - wl[i, h]) <= 2 * bl
 
 
+# ---- calls of more threads than a launch takes in one direction -------------------------------------------------------------------
+
+def test_more_rows_than_a_launch_has_threads_in_a_row(torch):
+    """Append and read of 2^29 + 77 tokens, eight threads to a row; a few of them have slots, at both ends."""
+    import zvdb_amd as zv
+    n, d = 2**29 + 77, 8
+    lay = zv.KVLayout(head_dim=d, kv_heads=1, page_size=16, pages=16)
+    slots = torch.full((n,), -1, dtype=torch.int64, device="cuda")
+    slots[:100], slots[-100:] = torch.arange(100, device="cuda"), torch.arange(100, 200, device="cuda")
+    k = torch.zeros((n, d), dtype=torch.bfloat16, device="cuda")
+    k[:100], k[-100:] = (torch.randn(100, d, device="cuda") for _ in range(2))
+    few, rows = torch.cat((slots[:100], slots[-100:])), torch.cat((k[:100], k[-100:]))
+    cache, want = (torch.zeros(lay.pages * lay.page_bytes, dtype=torch.uint8, device="cuda") for _ in range(2))
+    lay.append_dev(cache.data_ptr(), k.data_ptr(), d, k.data_ptr(), d, zv.KV_BF16, n, slots.data_ptr(), stream(torch))
+    lay.append_dev(want.data_ptr(), rows.data_ptr(), d, rows.data_ptr(), d, zv.KV_BF16, 200, few.data_ptr(), stream(torch))
+    assert torch.equal(cache, want)
+    a, b = torch.empty_like(rows), torch.empty_like(rows)
+    lay.read_dev(want.data_ptr(), few.data_ptr(), 200, a.data_ptr(), b.data_ptr(), zv.KV_BF16, stream(torch))
+    out = k.fill_(3.0)
+    for at in ((out.data_ptr(), 0), (0, out.data_ptr())):
+        out.fill_(3.0)
+        lay.read_dev(cache.data_ptr(), slots.data_ptr(), n, *at, zv.KV_BF16, stream(torch))
+        assert torch.equal(torch.cat((out[:100], out[-100:])), a if at[0] else b) and not out[100:-100].any()
+
+
+@pytest.mark.parametrize("n,heads,group,max_new", [(2**21 + 3, 8, 1, 1), (16_384, 8, 8, 2_064)])  # single tokens; one long prompt among them
+def test_more_requests_than_a_launch_has_threads_in_a_row(torch, n, heads, group, max_new):
+    """One memory that all requests read, each some of its tokens; halves of the call are bit for bit the same."""
+    import zvdb_amd as zv
+    d, qh, typ = 64, heads * group, kv_type("bf16")
+    rng = np.random.default_rng(51)
+    mem = Memory(torch, rng, [max_new + 40], d, heads, 16)
+    gen = torch.Generator("cuda").manual_seed(52)
+    new = torch.ones(n, dtype=torch.int32, device="cuda")
+    new[n // 3] = max_new
+    lengths = new + torch.randint(0, 40, (n,), generator=gen, device="cuda", dtype=torch.int32)
+    starts = torch.cat((new.new_zeros(1), torch.cumsum(new, 0).int()))
+    tables = mem.i32(mem.tables).expand(n, -1).contiguous()
+    rows, max_length = int(starts[-1]), max_new + 40
+    q = torch.randn((rows, qh, d), generator=gen, device="cuda").to(torch.bfloat16)
+
+    def call(first, last):
+        at, to = int(starts[first]), int(starts[last])
+        out = torch.full((to - at + 1, qh, d), 77.0, dtype=torch.bfloat16, device="cuda")
+        lse = torch.full((to - at + 1, qh), 77.0, device="cuda")
+        own = starts[first:last + 1] - starts[first]
+        assert mem.lay.attend_workspace(typ, qh, last - first, to - at, max_new, max_length) == 0
+        mem.lay.attend_dev(mem.cache.data_ptr(), q[at:].data_ptr(), qh * d, typ, qh, last - first, own.data_ptr(), to - at, max_new, lengths[first:].data_ptr(),
+                           tables[first:].data_ptr(), mem.stride, max_length, 0.125, True, 0, 0, out.data_ptr(), lse.data_ptr(), stream(torch))
+        torch.cuda.synchronize()
+        assert (out[-1] == 77.0).all() and (lse[-1] == 77.0).all()
+        return out[:-1], lse[:-1]
+
+    whole, parts = call(0, n), [call(0, n // 2), call(n // 2, n)]
+    for x, y in zip(whole, zip(*parts)):
+        assert torch.equal(x, torch.cat(y))
+    for i in (0, n // 3, n - 1):  # and some rows against the definition
+        r, length = int(starts[i + 1]) - 1, int(lengths[i])
+        for h in (0, qh - 1):
+            o, l, bo, bl = ref.attend_row(q[r, h].double().cpu().numpy(), mem.k[:length, h // group], mem.v[:length, h // group], 0.125, "bf16")
+            assert (np.abs(whole[0][r, h].double().cpu().numpy() - o) <= bo).all() and abs(float(whole[1][r, h]) - l) <= bl
+
+
+def test_more_lists_than_a_launch_has_threads_in_a_row(torch):
+    n, heads, d, k = 2**21 + 3, 8, 64, 2
+    mem = Memory(torch, np.random.default_rng(53), [60], d, heads, 16)
+    gen = torch.Generator("cuda").manual_seed(54)
+    q = torch.randn((n, heads, d), generator=gen, device="cuda").to(torch.bfloat16)
+    ids = torch.randint(0, 60, (heads, n, k), generator=gen, device="cuda")
+    lengths, tables = torch.full((n,), 60, dtype=torch.int32, device="cuda"), mem.i32(mem.tables).expand(n, -1).contiguous()
+
+    def call(first, last):
+        m, own = last - first, ids[:, first:last].contiguous()
+        out = torch.full((m + 1, heads, d), 77.0, dtype=torch.bfloat16, device="cuda")
+        lse = torch.full((m + 1, heads), 77.0, device="cuda")
+        mem.lay.attend_selected_dev(mem.cache.data_ptr(), q[first:].data_ptr(), heads * d, kv_type("bf16"), heads, m, own.data_ptr(), 0, k, lengths.data_ptr(), tables.data_ptr(),
+                                    mem.stride, 0.125, out.data_ptr(), lse.data_ptr(), stream(torch))
+        torch.cuda.synchronize()
+        assert (out[-1] == 77.0).all() and (lse[-1] == 77.0).all()
+        return out[:-1], lse[:-1]
+
+    whole, parts = call(0, n), [call(0, n // 2), call(n // 2, n)]
+    for x, y in zip(whole, zip(*parts)):
+        assert torch.equal(x, torch.cat(y)) and torch.isfinite(x).all()
+
+
 # ---- the calls together -----------------------------------------------------------------------------------------------------------
 
 class Server:

@@ -411,12 +411,13 @@ struct KvJoin {
 struct KvWhere {  // what the block's number says: known before anything is read
     uint32_t head, i, split, tile;
     __device__ explicit KvWhere(const KvAttendArgs &a) {
-        const uint32_t b = blockIdx.x / a.g.heads, turn = b / a.n;
-        head = blockIdx.x % a.g.heads;
+        const uint32_t b = kv_block() / a.g.heads, turn = b / a.n;
+        head = kv_block() % a.g.heads;
         i = (b + turn) % a.n;
         split = turn % a.splits;
-        tile = a.tiles - 1 - turn / a.splits;
+        tile = a.tiles - 1 - turn / a.splits;  // (from tiles on, wrapped: a block behind the last one)
     }
+    __device__ bool there(const KvAttendArgs &a) const { return tile < a.tiles; }
 };
 
 // The same for up to 64 requests where blocks are more than units: the blocks of tiles that no request has come last instead of first, where
@@ -431,7 +432,7 @@ struct KvWhere {  // what the block's number says: known before anything is read
 // 197 x 16 rows at width 256, fp32, 400 blocks: 53, 85; 70 blocks of short prompts: 10.6, 10.1).
 template <uint32_t ROWS>
 __device__ inline bool find_tile(const KvAttendArgs &a, KvWhere &where) {
-    const uint32_t lane = threadIdx.x & 63, rank = blockIdx.x / a.g.heads;
+    const uint32_t lane = threadIdx.x & 63, rank = kv_block() / a.g.heads;
     uint32_t tiles = 0, seeing = 0, reach = 0;  // row tiles, tokens whose rows these are, tokens that can be read
     int64_t base = 0;
     if (lane < a.n) {
@@ -596,6 +597,7 @@ __global__ __launch_bounds__(64 * WAVES, NB == 8 && TERMS == 3 ? 1 : NB == 8 || 
     constexpr uint32_t STRIDE = 32 * WAVES;
     const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4;
     const KvWhere where(a);
+    if (!where.there(a)) return;
     const uint32_t from = where.split * a.split_tokens, t0 = from + 32 * wave;  // the chunks of 32 go round the waves
     KvPages<32, STRIDE> pages(a, where.i, t0);                                     // (on their way together with the lengths)
     const KvBlock blk(a, where, 16);
@@ -702,7 +704,7 @@ __global__ __launch_bounds__(256, NB == 8 && TERMS == 3 ? 1 : 2) void k_kv_atten
     __shared__ uint4 keys[2][TILES][NB][64], vals[2][TILES / 2][2 * NB][64];
     const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4;
     KvWhere where(a);
-    if (a.by_tile && !find_tile<64 * NT>(a, where)) return;
+    if (a.by_tile ? !find_tile<64 * NT>(a, where) : !where.there(a)) return;
     const uint32_t t0 = where.split * a.split_tokens;
     KvPages<T, T> pages(a, where.i, t0);
     const KvBlock blk(a, where, 64 * NT);
@@ -954,7 +956,8 @@ __global__ __launch_bounds__(256, NB == 8 && TERMS == 3 ? 1 : NB == 8 || TERMS =
     } lds;
     uint64_t *const places = lds.places;
     const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4;
-    const uint32_t head = blockIdx.x % a.g.heads, b = blockIdx.x / a.g.heads, i = b % a.n, tile = b / a.n;
+    const uint32_t head = kv_block() % a.g.heads, b = kv_block() / a.g.heads, i = b % a.n, tile = b / a.n;
+    if (tile * 16 >= a.group) return;
     const uint64_t list = (uint64_t)head * a.n + i;
     const uint64_t *ids = a.ids + list * a.k;
     constexpr uint32_t AHEAD = kSelPass / 256;
@@ -1094,7 +1097,7 @@ static KvCut kv_cut(const KvGeom &g, uint32_t type, uint32_t group, uint32_t n, 
 
 template <int NB, int TERMS>
 static void launch_attend_as(const KvAttendArgs &a, const KvCut &c, hipStream_t s) {
-    const dim3 grid((uint32_t)c.blocks), block(64 * c.waves);
+    const dim3 grid = kv_grid(c.blocks), block(64 * c.waves);
     if (c.wide && c.nt == 3) hipLaunchKernelGGL((k_kv_attend_wide<NB, wide_tiles(NB, TERMS), TERMS>), grid, block, 0, s, a);
     else if (c.wide && c.nt == 2) hipLaunchKernelGGL((k_kv_attend_wide<NB, NB == 8 ? 1 : 2, TERMS>), grid, block, 0, s, a);
     else if (c.wide) hipLaunchKernelGGL((k_kv_attend_wide<NB, 1, TERMS>), grid, block, 0, s, a);
@@ -1120,8 +1123,8 @@ static void launch_join(const KvAttendArgs &a, uint32_t blocks, uint32_t type, h
 
 template <int NB>
 static void launch_selected(const KvAttendArgs &a, uint32_t blocks, uint32_t type, hipStream_t s) {
-    if (type == ZVDB_KV_F32) hipLaunchKernelGGL((k_kv_attend_selected<NB, 3>), dim3(blocks), dim3(256), 0, s, a);
-    else hipLaunchKernelGGL((k_kv_attend_selected<NB, 1>), dim3(blocks), dim3(256), 0, s, a);
+    if (type == ZVDB_KV_F32) hipLaunchKernelGGL((k_kv_attend_selected<NB, 3>), kv_grid(blocks), dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((k_kv_attend_selected<NB, 1>), kv_grid(blocks), dim3(256), 0, s, a);
 }
 
 static int check_queries(const KvGeom &g, const void *q, uint64_t q_stride, uint32_t type, uint32_t q_heads, float scale, const void *out, const void *cache) {
@@ -1219,11 +1222,10 @@ int zvdb_hip_kv_attend_dev(const zvdb_hip_kv_layout *layout, const void *d_cache
     else launch_attend<8>(a, c, type, s);
     ZV_HIP(hipGetLastError());
     if (c.splits > 1) {
-        const uint64_t blocks = (uint64_t)q_heads * n * max_new;
-        KV_ARG(blocks < 0x7FFFFFFFull, "kv_attend: the call is too large (%llu rows)", (unsigned long long)blocks);
-        if (w == 64) launch_join<64>(a, (uint32_t)blocks, type, s);
-        else if (w == 128) launch_join<128>(a, (uint32_t)blocks, type, s);
-        else launch_join<256>(a, (uint32_t)blocks, type, s);
+        const uint32_t blocks = q_heads * n * max_new;  // (a call in splits has fewer than two tiles of rows for each unit)
+        if (w == 64) launch_join<64>(a, blocks, type, s);
+        else if (w == 128) launch_join<128>(a, blocks, type, s);
+        else launch_join<256>(a, blocks, type, s);
         ZV_HIP(hipGetLastError());
     }
     return ZVDB_OK;

@@ -52,9 +52,18 @@ class KvDevice {
 constexpr uint64_t kKvStrideEnd = 1ull << 40;
 inline bool kv_stride_ok(uint64_t stride, uint64_t row) { return stride >= row && stride < kKvStrideEnd && stride % 8 == 0; }
 
+// A launch has fewer than 2^32 threads in a direction: blocks from 2^kGridShift on go on in y, and kv_block() counts them all.  The last
+// row of y is launched whole, so that a kernel meets blocks behind its last one.
+constexpr uint32_t kGridShift = 22;
+inline dim3 kv_grid(uint64_t blocks, uint32_t z = 1) {
+    return blocks <= 1u << kGridShift ? dim3((uint32_t)blocks, 1, z) : dim3(1u << kGridShift, (uint32_t)((blocks - 1) >> kGridShift) + 1, z);
+}
+
 inline bool kv_aligned(const void *p, uintptr_t a) { return reinterpret_cast<uintptr_t>(p) % a == 0; }
 
 #if defined(__HIPCC__)
+__device__ inline uint32_t kv_block() { return blockIdx.y << kGridShift | blockIdx.x; }
+
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));

@@ -233,12 +233,12 @@ template <class T, int NB>
 __global__ __launch_bounds__(256) void k_kv_append(uint8_t *cache, const KvGeom g, const T *k, uint64_t k_stride, const T *v, uint64_t v_stride,
                                                    const uint64_t *slots, uint32_t n) {
     constexpr uint32_t L = 4 * NB;  // lanes of a row
-    const uint32_t c8 = threadIdx.x % L, groups = (g.heads + kAppendHeads - 1) / kAppendHeads, head0 = blockIdx.x % groups * kAppendHeads;
-    const uint64_t i = (uint64_t)(blockIdx.x / groups) * (256 / L) + threadIdx.x / L;
+    const uint32_t c8 = threadIdx.x % L, groups = (g.heads + kAppendHeads - 1) / kAppendHeads, head0 = kv_block() % groups * kAppendHeads;
+    const uint64_t i = (uint64_t)(kv_block() / groups) * (256 / L) + threadIdx.x / L;
     if (i >= n) return;  // (whole rows leave: the four lanes of a block stay together)
     const uint64_t slot = slots[i];
     if (slot >= (uint64_t)g.pages << g.page_shift) return;
-    const bool value = blockIdx.y;
+    const bool value = blockIdx.z;
     const T *src = (value ? v + i * v_stride : k + i * k_stride) + (uint64_t)head0 * g.dim + c8 * 8;
     float x[kAppendHeads][8] = {};
 #pragma unroll
@@ -309,9 +309,9 @@ constexpr int kReadHeads = 4;
 template <class T, int NB>
 __global__ __launch_bounds__(256) void k_kv_read(const uint8_t *cache, const KvGeom g, const uint64_t *slots, uint32_t n, T *k, T *v) {
     constexpr uint32_t E = 16 / sizeof(T), L = 32 * NB / E;  // elements of a lane, lanes of a row
-    const uint32_t col = threadIdx.x % L * E, groups = (g.heads + kReadHeads - 1) / kReadHeads, head0 = blockIdx.x % groups * kReadHeads;
-    const uint64_t i = (uint64_t)(blockIdx.x / groups) * (256 / L) + threadIdx.x / L;
-    const bool value = k == nullptr || blockIdx.y;
+    const uint32_t col = threadIdx.x % L * E, groups = (g.heads + kReadHeads - 1) / kReadHeads, head0 = kv_block() % groups * kReadHeads;
+    const uint64_t i = (uint64_t)(kv_block() / groups) * (256 / L) + threadIdx.x / L;
+    const bool value = k == nullptr || blockIdx.z;
     T *const dst = value ? v : k;
     if (i >= n || col >= g.dim) return;
     const uint64_t slot = slots[i];
@@ -355,7 +355,7 @@ template <class T>
 static void launch_append(uint8_t *cache, const KvGeom &g, const void *k, uint64_t ks, const void *v, uint64_t vs, const uint64_t *slots, uint32_t n, hipStream_t s) {
     const T *kk = static_cast<const T *>(k), *vv = static_cast<const T *>(v);
     const uint32_t w = kv_width(g.dim), rows = 256 / (w / 8);
-    const dim3 grid((uint32_t)(((uint64_t)n + rows - 1) / rows * ((g.heads + kAppendHeads - 1) / kAppendHeads)), 2);
+    const dim3 grid = kv_grid(((uint64_t)n + rows - 1) / rows * ((g.heads + kAppendHeads - 1) / kAppendHeads), 2);
     if (w == 64) hipLaunchKernelGGL((k_kv_append<T, 2>), grid, dim3(256), 0, s, cache, g, kk, ks, vv, vs, slots, n);
     else if (w == 128) hipLaunchKernelGGL((k_kv_append<T, 4>), grid, dim3(256), 0, s, cache, g, kk, ks, vv, vs, slots, n);
     else hipLaunchKernelGGL((k_kv_append<T, 8>), grid, dim3(256), 0, s, cache, g, kk, ks, vv, vs, slots, n);
@@ -365,7 +365,7 @@ template <class T>
 static void launch_read(const uint8_t *cache, const KvGeom &g, const uint64_t *slots, uint32_t n, void *k, void *v, hipStream_t s) {
     T *kk = static_cast<T *>(k), *vv = static_cast<T *>(v);
     const uint32_t w = kv_width(g.dim), rows = 256 * 16 / sizeof(T) / w, groups = (g.heads + kReadHeads - 1) / kReadHeads;
-    const dim3 grid((uint32_t)(((uint64_t)n + rows - 1) / rows * groups), k && v ? 2 : 1);
+    const dim3 grid = kv_grid(((uint64_t)n + rows - 1) / rows * groups, k && v ? 2 : 1);
     if (w == 64) hipLaunchKernelGGL((k_kv_read<T, 2>), grid, dim3(256), 0, s, cache, g, slots, n, kk, vv);
     else if (w == 128) hipLaunchKernelGGL((k_kv_read<T, 4>), grid, dim3(256), 0, s, cache, g, slots, n, kk, vv);
     else hipLaunchKernelGGL((k_kv_read<T, 8>), grid, dim3(256), 0, s, cache, g, slots, n, kk, vv);
