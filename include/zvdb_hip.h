@@ -501,7 +501,8 @@ int zvdb_hip_kv_read_dev(const zvdb_hip_kv_layout *layout, const void *d_cache, 
  * Rows behind d_starts[n] stay as they are.  max_new and max_length are bounds that the host knows: what exceeds them is not
  * computed, or not seen.  With ZVDB_KV_BF16 the probabilities are rounded to bf16 for their product with V; with ZVDB_KV_F32 queries and
  * probabilities keep 24 bits.  Same inputs, same bits.  The workspace (zvdb_hip_kv_attend_workspace for the same sizes, on the same
- * kind of device) belongs to one call at a time. */
+ * kind of device) belongs to one call at a time.  Fewer requests or rows may need MORE of it: fewer blocks are cut into more splits.  A
+ * buffer for calls of several sizes takes the largest of their answers (the query launches nothing); one that is too small is refused. */
 int zvdb_hip_kv_attend_workspace(const zvdb_hip_kv_layout *layout, uint32_t type, uint32_t q_heads, uint32_t n, uint32_t rows, uint32_t max_new, uint32_t max_length,
                                  uint64_t *out_bytes);
 int zvdb_hip_kv_attend_dev(const zvdb_hip_kv_layout *layout, const void *d_cache, const void *d_q, uint64_t q_stride, uint32_t type, uint32_t q_heads, uint32_t n,

@@ -596,6 +596,34 @@ def test_a_workspace_that_is_too_small_is_refused(torch):
         assert e.value.code == 1
 
 
+def test_one_workspace_for_batches_of_every_size(torch):
+    """The need does not grow with the batch: the largest answer over the sizes in use serves them all, the largest batch's alone does not."""
+    import zvdb_amd as zv
+    rng = np.random.default_rng(61)
+    mem = Memory(torch, rng, [40 + 37 * (i % 31) for i in range(64)], 64, 8, 16)
+    q, qx = as_type(torch, rng.standard_normal((64, 8, 64)), "bf16")
+    sizes = {n: mem.lay.attend_workspace(zv.KV_BF16, 8, n, n, 1, 8192) for n in range(1, 65)}
+    assert sizes[64] == 0 and max(sizes.values()) == max(sizes[n] for n in range(1, 64)) > 0
+    ws = torch.full((max(sizes.values()),), 255, dtype=torch.uint8, device="cuda")
+    lengths, tables, starts = mem.i32(mem.lengths), mem.i32(mem.tables), mem.i32(range(65))
+    out, lse = torch.empty((64, 8, 64), dtype=torch.bfloat16, device="cuda"), torch.empty((64, 8), device="cuda")
+
+    def call(n, have):
+        mem.lay.attend_dev(mem.cache.data_ptr(), q.data_ptr(), 512, zv.KV_BF16, 8, n, starts.data_ptr(), n, 1, lengths.data_ptr(), tables.data_ptr(), mem.stride, 8192,
+                           0.125, True, ws.data_ptr(), have, out.data_ptr(), lse.data_ptr(), stream(torch))
+        torch.cuda.synchronize()
+
+    for n in (64, 63, 48, 33, 16, 5, 1):
+        out.fill_(77.0), lse.fill_(77.0)
+        call(n, ws.numel())
+        got, l = out.double().cpu().numpy(), lse.double().cpu().numpy()
+        check_rows(mem, got, l, qx, [(r, r) for r in range(0, n, 7)], 1, "bf16", 0.125, lambda r, i: slice(0, mem.lengths[i]))
+        assert (got[n:] == 77.0).all() and (got[:n] != 77.0).all()
+    with pytest.raises(zv.ZvdbError) as e:
+        call(16, sizes[64])
+    assert e.value.code == 1
+
+
 def test_host_memory_is_refused(torch):
     import zvdb_amd as zv
     lay = zv.KVLayout(head_dim=64, kv_heads=1, page_size=16, pages=1)

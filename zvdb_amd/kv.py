@@ -43,6 +43,8 @@ class KVLayout:
         check(self._L.zvdb_hip_kv_read_dev(self._p, cache_ptr, slots_ptr, n, k_ptr, v_ptr, type, stream))
 
     def attend_workspace(self, type: int, q_heads: int, n: int, rows: int, max_new: int, max_length: int) -> int:
+        """Bytes of workspace of attend_dev with these sizes.  Fewer requests or rows may need more: a buffer for calls of several sizes
+        takes the largest of their answers."""
         b = C.c_uint64(0)
         check(self._L.zvdb_hip_kv_attend_workspace(self._p, type, q_heads, n, rows, max_new, max_length, C.byref(b)))
         return b.value
