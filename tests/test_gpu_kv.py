@@ -401,6 +401,42 @@ def test_pages_that_are_none_hide_their_tokens(torch, kind, new):
 
 @pytest.mark.parametrize("kind", ["bf16", "fp32"])
 @pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("page", [16, 64])
+@pytest.mark.parametrize("n,heads,long,new", [
+    (512, 1, [4096 + 33, 8300], 1),                            # single tokens: 4,096 are what a wave knows the pages of at a time
+    (130, 1, [1024 + 33, 2500], 128), (64, 2, [1024 + 1, 2100], 130)])  # prompts: 1,024
+def test_long_contexts_that_are_not_split(torch, kind, d, page, n, heads, long, new):
+    """Requests of many pages beside many short ones: too many blocks for splits, so that one goes through all of its request's pages.  Pages
+    that are none, and NaN values, lie behind the first that it asks for."""
+    group, rng = 2, np.random.default_rng(d + n)
+    far = 4100 if new == 1 else 1030
+
+    def spoil(mem, k, v):
+        v[mem.first[1] + far + 20, 0, 7] = np.nan
+        v[mem.first[1] + long[1] - 1, heads - 1, d - 1] = np.inf
+
+    lengths = long + [i % 5 for i in range(n - 2)]
+    with np.errstate(invalid="ignore"):
+        mem = Memory(torch, rng, lengths, d, heads, page, spoil=spoil)
+    hide = {0: [far // page], 1: [far // page - 1, far // page + 4]}
+    tables = mem.tables.copy()
+    for i, ps in hide.items():
+        tables[i, ps] = mem.pages
+    count = [new, new] + [min(x, 2) for x in lengths[2:]]
+    starts = np.concatenate(([0], np.cumsum(count))).astype(int)
+    q, qx = as_type(torch, rng.standard_normal((starts[-1], heads * group, d)), kind)
+    got, lse, size = attend(mem, q, count, group, kind, True, 0.125, tables=tables)
+    assert size == 0
+
+    def visible(r, i):
+        return np.array([t for t in range(lengths[i] - count[i] + r - starts[i] + 1) if t // page not in hide.get(i, [])], dtype=int)
+
+    rows = [(0, 0), (new - 1, 0), (new, 1), (2 * new - 1, 1)] + [(starts[i], i) for i in (5, 6, n - 1) if count[i]]
+    check_rows(mem, got, lse, qx, rows, group, kind, 0.125, visible)
+
+
+@pytest.mark.parametrize("kind", ["bf16", "fp32"])
+@pytest.mark.parametrize("d", [64, 128, 256])
 def test_a_nan_reaches_the_rows_that_see_it_and_no_others(torch, kind, d):
     def spoil(mem, k, v):
         v[30, 0, 33] = np.nan         # one block of one value
@@ -720,6 +756,50 @@ def test_selected_rows(torch, kind, d, heads, group, page, k):
     for c in (counts, None):
         got, lse = selected(mem, q, ids, c, group, kind, 0.3)
         check_selected(mem, got, lse, qx, ids, c, group, kind, float(np.float32(0.3)))
+
+
+@pytest.mark.parametrize("kind", ["bf16", "fp32"])
+@pytest.mark.parametrize("d,k", [(64, 2049), (128, 1024), (128, 1100), (256, 1025), (256, 2100)])
+def test_long_lists_of_selected_rows(torch, kind, d, k):
+    """More entries than are resolved at a time, some that are not there, a NaN behind the first 1,024."""
+    rng = np.random.default_rng(d + k)
+    lengths = [1500, 700]
+
+    def spoil(mem, key, v):
+        v[mem.first[0] + 1499, 0, 9] = np.nan
+
+    mem = Memory(torch, rng, lengths, d, 2, 32, spoil=spoil)
+    ids = np.stack([np.stack([rng.integers(0, x - 1, k) for x in lengths]) for _ in range(2)]).astype(np.uint64)
+    ids[:, :, 5::11] = 2**64 - 1
+    ids[:, 1, 7::13] = 700
+    ids[0, 0, -1] = 1499
+    counts = np.array([[k, k - 1], [k - 20, k]])
+    q, qx = as_type(torch, rng.standard_normal((2, 4, d)), kind)
+    got, lse = selected(mem, q, ids, counts, 2, kind, 0.3)
+    assert np.isnan(got[0, 0, 9])
+    check_selected(mem, got, lse, qx, ids, counts, 2, kind, float(np.float32(0.3)))
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_selected_rows_beyond_32_bits_of_bytes(torch, d):
+    """Pages behind 4 GiB: the same answers as in a small cache."""
+    import zvdb_amd as zv
+    rng = np.random.default_rng(15)
+    mem = Memory(torch, rng, [300, 65], d, 2, 16)
+    big = zv.KVLayout(head_dim=d, kv_heads=2, page_size=16, pages=(10 << 30) // mem.lay.page_bytes)
+    far = torch.empty(big.pages * big.page_bytes, dtype=torch.uint8, device="cuda")
+    move = big.pages - mem.pages
+    far[move * big.page_bytes:] = mem.cache
+    ids = np.stack([np.stack([rng.permutation(300)[:60] for _ in range(2)]) for _ in range(2)]).astype(np.uint64)
+    for kind in ("bf16", "fp32"):
+        q, qx = as_type(torch, rng.standard_normal((2, 4, d)), kind)
+        want = selected(mem, q, ids, None, 2, kind, 0.1)
+        check_selected(mem, *want, qx, ids, None, 2, kind, float(np.float32(0.1)))
+        small = (mem.lay, mem.cache, mem.tables)
+        mem.lay, mem.cache, mem.tables = big, far, np.where(mem.tables < mem.pages, mem.tables + move, mem.tables).astype(np.uint32)
+        got = selected(mem, q, ids, None, 2, kind, 0.1)
+        mem.lay, mem.cache, mem.tables = small
+        assert np.array_equal(got[0], want[0]) and np.array_equal(got[1], want[1])
 
 
 def test_selected_rows_of_hidden_pages_and_nan(torch):
