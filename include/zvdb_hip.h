@@ -496,8 +496,8 @@ int zvdb_hip_kv_read_dev(const zvdb_hip_kv_layout *layout, const void *d_cache, 
  * max_new of them; d_starts as zvdb_hip_kv_plan_dev writes it) and d_lengths[i] tokens (at most max_length), its new ones included.
  * Query head h reads key/value head h / (q_heads / kv_heads).  causal: the j-th of m new tokens sees the tokens before position
  * length - m + j + 1; else all of them.  d_out [rows][q_heads][head_dim] of `type`, d_lse fp32 [rows][q_heads] (log of the sum of
- * exponentials; NULL: not wanted).  A row that sees nothing, or no score above -inf, gets 0 and -inf.  A NaN reaches the rows that see its
- * token and no others; values as large as a block can hold stay finite.
+ * exponentials; NULL: not wanted).  A row that sees nothing, or no score above -inf, gets 0 and -inf; one with a score over all of fp32 is
+ * NaN.  A NaN reaches the rows that see its token and no others; values as large as a block can hold stay finite.
  * Rows behind d_starts[n] stay as they are.  max_new and max_length are bounds that the host knows: what exceeds them is not
  * computed, or not seen.  With ZVDB_KV_BF16 the probabilities are rounded to bf16 for their product with V; with ZVDB_KV_F32 queries and
  * probabilities keep 24 bits.  Same inputs, same bits.  The workspace (zvdb_hip_kv_attend_workspace for the same sizes, on the same

@@ -554,6 +554,28 @@ def test_rows_whose_scores_are_all_minus_infinity(torch, kind, d, length, new, h
 
 
 @pytest.mark.parametrize("kind", ["bf16", "fp32"])
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("query,scale", [(3e38, 0.125), (4.0, 1e38)])  # a product, and a finite product's score, over all of fp32
+@pytest.mark.parametrize("length,new,heads", [(40, 1, 1), (2100, 1, 1), (40, 33, 2), (1500, 70, 2), (300, 280, 32)])
+def test_rows_with_a_score_over_all_of_fp32_are_nan(torch, kind, d, query, scale, length, new, heads):
+    """The last token that the first row sees has such a score, all others 0; rows of request 1, whose keys are 0, have their means."""
+    def spoil(mem, k, v):
+        k[:] = 0.0
+        k[length - new, :, 5] = 6.0
+
+    mem = Memory(torch, np.random.default_rng(d), [length, 50], d, heads, 16, spoil=spoil)
+    q = torch.zeros((new + 1, 2 * heads, d), dtype=torch.bfloat16 if kind == "bf16" else torch.float32, device="cuda")
+    q[:, :, 5] = query
+    got, lse, _ = attend(mem, q, [new, 1], 2, kind, True, scale)
+    assert np.isnan(got[:new]).all() and np.isnan(lse[:new]).all()
+    assert np.isfinite(got[new]).all() and np.abs(lse[new] - np.log(50)).max() < 1e-5
+    if new == 1:
+        ids = np.tile(np.arange(length, dtype=np.uint64), (heads, 2, 1))
+        got, lse = selected(mem, q, ids, None, 2, kind, scale)
+        assert np.isnan(got[0]).all() and np.isnan(lse[0]).all() and np.isfinite(got[1]).all()
+
+
+@pytest.mark.parametrize("kind", ["bf16", "fp32"])
 @pytest.mark.parametrize("d,heads", [(64, 16), (128, 16), (256, 32)])
 def test_values_near_the_largest_in_whole_prompts(torch, kind, d, heads):
     *_, size = check_sizes(torch, [400, 700], [300, 290], d, heads, 2, kind, False, few=4)

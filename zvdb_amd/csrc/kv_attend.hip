@@ -237,7 +237,7 @@ struct KvRows {
             for (int t = 0; t < NT; ++t) {
                 const float to = fmaxf(m[t], max_over_row(mx[t]) + lift), by = __builtin_amdgcn_exp2f(m[t] - to);
                 m[t] = to;
-                l[t] *= by;
+                l[t] = fmaf(l[t], by, to - to);  // (NaN where a score is over all of fp32: exp2 makes 0 of a finite one minus infinity)
 #pragma unroll
                 for (int i = 0; i < 2 * NB; ++i) o[t][i] *= by;
             }
@@ -349,8 +349,8 @@ __device__ inline uint32_t live_scales(bool there, uint32_t at, uint32_t t1) {
     return live == 4 ? ~0u : (1u << (8 * live)) - 1;
 }
 
-// 1 / l; 0 where nothing is seen, or no score above -inf (a NaN among them is in O already)
-__device__ inline float over_sum(float l) { return l > 0.0f ? 1.0f / l : 0.0f; }
+// 1 / l; 0 where nothing is seen, or no score above -inf
+__device__ inline float over_sum(float l) { return l == 0.0f ? 0.0f : 1.0f / l; }
 __device__ inline float lse_of(float m, float l) { return (m + __log2f(l)) * kLn2; }
 
 // Where the waves of a block that share 16 rows and have tokens of their own are joined: every wave leaves what it has, and after one
