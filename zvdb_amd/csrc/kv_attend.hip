@@ -423,13 +423,13 @@ struct KvWhere {  // what the block's number says: known before anything is read
 // The same for up to 64 requests where blocks are more than units: the blocks of tiles that no request has come last instead of first, where
 // they held the units for some us before the others began.  False: there is no such tile.  (All 64 lanes call this.)
 //
-// Split tiles are numbered in the order of the requests, split by split (2 prompts of 1,329 x 4 rows, not causal: 30 us, 48 in turns; 313 x
-// 3 rows over 4,300 tokens: 26.5, 30.3; no difference where all requests have as many).
+// Split tiles are numbered in the order of the requests, split by split (2 prompts of 1,329 x 4 rows, not causal: 29 us, 47 in turns; 313 x
+// 3 rows over 4,300 tokens: 25.6, 29.2; no difference where all requests have as many).
 //
 // Whole tiles go by length: block b takes the b-th longest of all requests, so that the last blocks to start are the shortest.  Each lane
 // counts the tiles of one request that end behind some token, and the token is searched for behind which no more than b of them end: some
-// 2 us at a block's start, worth it where units get blocks one after the other (4 prompts, 1,376 blocks: 245 us, 274 in turns; 2 requests of
-// 197 x 16 rows at width 256, fp32, 400 blocks: 53, 85; 70 blocks of short prompts: 10.6, 10.1).
+// 2 us at a block's start, worth it where units get blocks one after the other (4 prompts, 1,376 blocks: 248 us, 277 in turns; 2 requests of
+// 197 x 16 rows at width 256, fp32, 400 blocks: 54, 85; 16 short prompts: 17.4, 16.7).
 template <uint32_t ROWS>
 __device__ inline bool find_tile(const KvAttendArgs &a, KvWhere &where) {
     const uint32_t lane = threadIdx.x & 63, rank = kv_block() / a.g.heads;
@@ -682,7 +682,7 @@ __global__ __launch_bounds__(64 * WAVES, NB == 8 && TERMS == 3 ? 1 : NB == 8 || 
 }
 
 // Row tiles of a wave of k_kv_attend_wide, at most: what 256 registers hold, and at width 64 two, which leave room for more waves on a SIMD
-// (8 prompts of up to 1,000 tokens, 32 heads x 64: 30 us, 35 with three; fp32, 3 of up to 1,469: 93, 86 with three, but 4 of 2,048: 151, 185)
+// (8 prompts of up to 1,000 tokens, 32 heads x 64: 32 us, 36 with three; fp32, 3 of up to 1,469: 91, 83 with three, but 4 of 2,048: 151, 185)
 constexpr int wide_tiles(int nb, int terms) { return nb == 8 ? 1 : nb == 4 && terms == 1 ? 3 : 2; }
 
 // Many rows (prompts): each of a block's four waves has NT tiles of its own and all walk the same tokens.  A wave's tile of 16 tokens (at
@@ -827,8 +827,8 @@ __device__ inline bool joined_row(const KvAttendArgs &a, uint32_t at, uint64_t &
 }
 
 // Joins up to kFewSplits splits of a row: four columns to a thread, which reads every split's maximum and sum for itself.  All that it
-// reads is asked for at once and nothing is waited for twice, where k_kv_join has three barriers for a row (4,864 rows of 256 in four
-// splits: 8.4 us, 10.9 with k_kv_join; 1,536 of 128 in three: 4.0, 4.7).
+// reads is asked for at once and nothing is waited for twice, where k_kv_join has three barriers for a row (4,864 rows of 256 in seven
+// splits: 8.4 us, 2.4 less than with k_kv_join; 1,536 of 128 in three: 4.9, 0.8 less).
 constexpr uint32_t kFewSplits = 8;
 
 template <int W, int TERMS>
@@ -1043,21 +1043,22 @@ __global__ __launch_bounds__(256, NB == 8 && TERMS == 3 ? 1 : NB == 8 || TERMS =
 
 // ---- launches -----------------------------------------------------------------------------------------------------------
 
-// How a call is cut.  Rows of one (request, head) that fit 64 are few: blocks of 16 whose waves divide the tokens; more of them give
-// each wave its own tiles, as many as leave three blocks with rows for two units of the card (one prompt of 4,000 over 4,000, 16 heads: 218
-// us with two tiles, 264 with one, 258 with three; 8 prompts of up to 300 x 4 rows: 33 with one, 50 with three; 82 new tokens of 7 heads
-// over 2,452: 14.6 with one, 21.4 with three).  The total of the rows says how many blocks that is, where prompts are of many lengths.
+// How a call is cut (all forms measured: profiles/kv/cuts.txt).  Rows of one (request, head) that fit 64 are few: blocks of 16 whose waves
+// divide the tokens; more of them give each wave its own tiles, as many as leave three blocks with rows for two units of the card (one prompt
+// of 4,000 over 4,000, 16 heads: 218 us with two tiles, 266 with one, 260 with three; 8 prompts of up to 300 x 4 rows: 34 with one, 51 with
+// three; 82 new tokens of 7 heads over 2,452: 14 with one, 20 with three).  The total of the rows says how many blocks that is, where prompts are
+// of many lengths.
 //
 // Tokens are split where blocks are fewer than the card wants.  Each part costs its start (some 5 us of dependent reads), its rows in the
-// workspace and its place in the join.  Few rows: none up to 1,024 tokens (one request: 9.2 us, 11.6 in two), parts of at least 512 up to
-// 32 parts (16 requests to 4,000, fp32: 18 us, 23 with 1,024), of 1,024 beyond (one head over 131,072: 18 us, 22 with 512), up to four
-// blocks for each unit unless there are two (requests differ in length, a good third of the splits is empty: 48 requests to 8,192 tokens:
-// 2 / 3 / 5 splits 58.5 / 53.4 / 59.8 us; 64 of 2,048: whole 29.8, two splits 39.8); at width 256, where a unit holds one block or two, up
-// to one (24 requests to 11,000, fp32: 35 us, 43 with four; 64 to 2,000: 22, 25).  Many: none from one block a unit on (7 prompts of 1,294
-// tokens, 294 blocks: 35 us, with four splits 82), else to two, four at width 256 with bf16 queries, whose blocks are the slowest (33 rows
-// of 8 heads over 4,100 tokens: 49 us, 65 with two, 66 with six; fp32, one block resident on a unit: 4 prompts of 422 x 5 rows over 1,415:
-// 37 us, 48 with four).  Few rows that leave units empty even so get eight waves to a block (one request of 1,024 tokens: 9.0 us, 12.8 with
-// four waves and splits).
+// workspace and its place in the join.  Few rows: none up to 1,024 tokens (one request: 9.7 us, 12.6 in two), parts of at least 512 up to
+// 32 parts (16 requests to 4,000, 32 heads x 64, fp32: 15.6 us, 17.4 with 1,024; x 128: 23.9, 22.1), of 1,024 beyond (one head over 131,072: 16.1
+// us, 19.0 with 2,048, 16.6 with 512), up to four blocks for each unit unless there are two (requests differ in length, a good third of the
+// splits is empty: 48 requests to 8,192 tokens: 2 / 3 / 5 splits 58.0 / 53.8 / 57.4 us; 64 of 2,048: whole 30, two splits 38); at width 256,
+// where a unit holds one block or two, up to one (24 requests to 11,000, fp32: 36 us, 46 with four; 64 to 2,000: 33 whole, 49).  Many: none
+// from one block a unit on (7 prompts of 1,294 tokens, 294 blocks: 33 us, with four splits 50), else to two, four at width 256 with bf16 queries,
+// whose blocks are the slowest (33 rows of 8 heads over 4,100 tokens: 50 us, 65 with two, 64 with six; fp32, one block resident on a unit: 4
+// prompts of 422 x 5 rows over 1,415: 37 us, 46 with four).  Few rows that leave units empty even so get eight waves to a block (one request of
+// 1,024 tokens: 9.7 us, 10.1 with four waves, 12.6 with four waves and splits).
 struct KvCut {
     bool wide, by_tile;
     uint32_t nt, tiles, splits, split_tokens, waves;
